@@ -16,9 +16,14 @@ from .runtime import (  # noqa: F401
     VARIANT_NCCL,
     VARIANT_OVERLAP,
     LAMB_REF_QUIRK,
+    QUANT_BLOCK,
     group,
     lib,
     library_path,
+    quant_decode,
+    quant_slice_elems,
+    quant_state,
+    quant_tensor_place,
     rendezvous_address,
     scattered_slice_elems,
     scattered_tensor_place,
@@ -28,6 +33,7 @@ from .runtime import (  # noqa: F401
 
 __all__ = [
     "CocoError", "Communicator", "HostBootstrap", "TensorList", "VARIANT_DSL", "VARIANT_NCCL", "VARIANT_OVERLAP",
-    "LAMB_REF_QUIRK", "group", "lib", "library_path", "rendezvous_address", "scattered_slice_elems", "scattered_tensor_place",
+    "LAMB_REF_QUIRK", "QUANT_BLOCK", "group", "lib", "library_path", "quant_decode", "quant_slice_elems", "quant_state",
+    "quant_tensor_place", "rendezvous_address", "scattered_slice_elems", "scattered_tensor_place",
     "slice_bounds", "topology_check",
 ]

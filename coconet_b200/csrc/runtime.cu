@@ -28,6 +28,7 @@
 #include "coconet_rt.h"
 #include "coconet_fused_generic.cuh"
 #include "fused_step.cuh"
+#include "list_step.cuh"
 
 using namespace coco;
 
@@ -116,6 +117,39 @@ struct IpcBlob {
   int pad;
 };
 
+// A call of the AdamW / gradient-norm family over a list of tensors.  The
+// arrays are the caller's; a call that waits for its group keeps copies.
+struct ListCall {
+  int op = 0;  // kListAdamW ...
+  size_t n = 0;
+  cocoDataType_t g_type = cocoFloat32, lp_type = cocoFloat16;
+  const void *const *g = nullptr;
+  float *const *w = nullptr;
+  void *const *lp = nullptr;            // or null: no copies
+  const unsigned char *no_decay = nullptr;  // or null: every tensor decays
+  const size_t *counts = nullptr;
+  AdamWArgs adam = {};                  // scalars, state and norm pointers
+  NormArgs norm = {};
+  cudaStream_t stream = nullptr;
+};
+struct OwnedListCall {
+  ListCall call;
+  std::vector<const void *> g;
+  std::vector<float *> w;
+  std::vector<void *> lp;
+  std::vector<unsigned char> no_decay;
+  std::vector<size_t> counts;
+  explicit OwnedListCall(const ListCall &c) : call(c), g(c.g, c.g + c.n), counts(c.counts, c.counts + c.n) {
+    if (c.w) w.assign(c.w, c.w + c.n);
+    if (c.lp) lp.assign(c.lp, c.lp + c.n);
+    if (c.no_decay) no_decay.assign(c.no_decay, c.no_decay + c.n);
+    call.g = g.data(), call.counts = counts.data();
+    call.w = c.w ? w.data() : nullptr;
+    call.lp = c.lp ? lp.data() : nullptr;
+    call.no_decay = c.no_decay ? no_decay.data() : nullptr;
+  }
+};
+
 // One fused call waiting for its launch (single-process groups).
 struct PendingCall {
   int opt = 0;
@@ -133,6 +167,7 @@ struct PendingCall {
   std::vector<const void *> sg;
   std::vector<float *> sw;
   std::vector<size_t> scounts;
+  std::shared_ptr<OwnedListCall> list;  // AdamW / gradient norm over a list, else null
 };
 
 // Flat layout of a list of tensors: each tensor starts at a multiple of 8
@@ -144,16 +179,18 @@ struct FlatLayout {
   size_t total = 0;
   size_t slice = 0;
 };
-FlatLayout flat_layout(const size_t *counts, size_t n, int world) {
+// `align` elements instead of 8 for moments in 8 bits: blocks that share a
+// scale are never cut by a tensor's end or a slice's.
+FlatLayout flat_layout(const size_t *counts, size_t n, int world, size_t align = 8) {
   FlatLayout L;
   L.off.resize(n);
   size_t at = 0;
   for (size_t b = 0; b < n; ++b) {
     L.off[b] = at;
-    at += (counts[b] + 7) / 8 * 8;
+    at += (counts[b] + align - 1) / align * align;
   }
   L.total = at;
-  L.slice = ((at + world - 1) / world + 7) / 8 * 8;
+  L.slice = ((at + world - 1) / world + align - 1) / align * align;
   return L;
 }
 
@@ -189,6 +226,8 @@ struct cocoComm {
   size_t seg_cap = 0;
   double *seg_part = nullptr;      // scattered LAMB: per-segment, per-CTA partial sums
   size_t seg_part_cap = 0;         // in doubles
+  char *list_dev = nullptr;        // AdamW / norm over a list at world sizes above 1: the ranks' pieces
+  size_t list_cap = 0;             // in bytes
   int ctas_per_sm = 0;  // 0 = automatic
   int threads = 512;
   int timeout_ms = 10000;
@@ -629,12 +668,24 @@ int launch_single(cocoComm *c, const PendingCall &pc, char *const g_views[],
 
 // Launch every queued call of a single-process group: one launch per device;
 // ranks that share a device become virtual ranks of one cooperative launch.
+int flush_list_group(LocalGroup *grp);
+
 int flush_group(LocalGroup *grp) {
   std::lock_guard<std::mutex> lock(grp->mu);
   const int R = (int)grp->comms.size();
   for (cocoComm *c : grp->comms)
     if (!c->has_pending) return cocoInvalidUsage;  // every rank must have called
   const PendingCall &first = grp->comms[0]->pending;
+  for (cocoComm *c : grp->comms)
+    if ((c->pending.list != nullptr) != (first.list != nullptr)) {
+      for (cocoComm *o : grp->comms) o->has_pending = false;
+      return cocoInvalidUsage;  // ranks disagree on the operation
+    }
+  if (first.list) {
+    const int rc = flush_list_group(grp);
+    for (cocoComm *c : grp->comms) c->has_pending = false, c->pending.list.reset();
+    return rc;
+  }
   char *g_views[kMaxRanks], *out_views[kMaxRanks];
   FlagPage *flags[kMaxRanks];
   for (int r = 0; r < R; ++r) {
@@ -780,18 +831,361 @@ int flush_group(LocalGroup *grp) {
 // free when none is.  COCO_NVTX=0 switches it off.
 struct NvtxRange {
   bool on;
-  explicit NvtxRange(const PendingCall &pc) {
+  explicit NvtxRange(const char *name) {
     static const bool enabled = env_int("COCO_NVTX", 1) != 0;
     on = enabled;
-    if (on)
-      nvtxRangePushA(pc.coll ? "coconet collective"
-                     : pc.opt == kSGD ? "coconet fused SGD"
-                     : pc.opt == kAdam ? "coconet fused Adam" : "coconet fused LAMB");
+    if (on) nvtxRangePushA(name);
   }
+  explicit NvtxRange(const PendingCall &pc)
+      : NvtxRange(pc.coll ? "coconet collective"
+                  : pc.opt == kSGD ? "coconet fused SGD"
+                  : pc.opt == kAdam ? "coconet fused Adam" : "coconet fused LAMB") {}
   ~NvtxRange() {
     if (on) nvtxRangePop();
   }
 };
+
+// ---- AdamW and the gradient norm over a list ---------------------------------
+// At world sizes above 1 a call carries a sequence number and uploads a table,
+// neither of which a replay could repeat.
+int refuse_capture(const cocoComm *c, cudaStream_t stream) {
+  cudaStreamCaptureStatus st = cudaStreamCaptureStatusNone;
+  DeviceGuard guard(c->device);
+  if (!guard.ok) return cocoCudaError;
+  CUDA_TRY(cudaStreamIsCapturing(stream, &st));
+  return st == cudaStreamCaptureStatusNone ? cocoSuccess : cocoInvalidUsage;
+}
+
+size_t list_align(int op) { return op == kListAdamWQuant ? kListUnit : kListGroup; }
+
+// A list's largest launch in groups: the kernels count them in 32 bits.
+constexpr size_t kListMaxGroups = (size_t)1 << 31;
+
+int ctas_for(const cocoComm *c, size_t units, int threads, int per_sm) {
+  if (c->ctas_per_sm > 0) per_sm = std::min(per_sm, c->ctas_per_sm);
+  const size_t warps = (size_t)threads / 32;
+  const size_t need = std::max<size_t>(1, (units + warps - 1) / warps);
+  return (int)std::min<size_t>({need, (size_t)per_sm * c->sm_count, (size_t)kMaxCtasPerRank});
+}
+
+// World size 1, AdamW: the list in one or several parameter-borne tables.
+template <int CAP> int launch_adamw_local(cocoComm *c, const ListCall &lc) {
+  const bool quant = lc.op == kListAdamWQuant;
+  const size_t align_groups = list_align(lc.op) / kListGroup;
+  const size_t state_bytes = quant ? 1 : sizeof(float);
+  const int threads = adamw_threads(quant, lc.g_type), per_sm = adamw_ctas_per_sm(quant, lc.g_type);
+  static thread_local ListTable<CAP> tab;
+  AdamWArgs a = lc.adam;
+  size_t groups_before = 0;
+  size_t b = 0;
+  while (b < lc.n) {
+    int n = 0;
+    size_t at = 0;
+    for (; b < lc.n && n < CAP; ++b) {
+      const size_t count = lc.counts[b];
+      if (count == 0) continue;
+      const size_t len = (count + list_align(lc.op) - 1) / list_align(lc.op) * align_groups;
+      if (n > 0 && at + len > kListMaxGroups) break;
+      tab.g[n] = lc.g[b];
+      tab.w[n] = lc.w[b];
+      tab.lp[n] = lc.lp ? lc.lp[b] : nullptr;
+      tab.off[n] = (unsigned)at;
+      tab.missing[n] = (unsigned char)(len * kListGroup - count);
+      tab.decays[n] = !(lc.no_decay && lc.no_decay[b]);
+      at += len;
+      ++n;
+    }
+    if (n == 0) break;
+    tab.off[n] = (unsigned)at;
+    a.n = n;
+    a.m = (char *)lc.adam.m + groups_before * kListGroup * state_bytes;
+    a.v = (char *)lc.adam.v + groups_before * kListGroup * state_bytes;
+    a.scale = quant ? lc.adam.scale + groups_before / kListUnitGroups * 2 : nullptr;
+    a.flat0 = groups_before * kListGroup;
+    const size_t units = (at + kListUnitGroups - 1) / kListUnitGroups;
+    CUDA_TRY(launch_adamw<CAP>(quant, lc.g_type, tab, a, ctas_for(c, units, threads, per_sm), lc.stream));
+    c->launches++;
+    groups_before += at;
+  }
+  return cocoSuccess;
+}
+
+// World size 1, norm: 16-byte groups by address; a tensor longer than a launch
+// can count is entered in parts.
+template <int CAP> int launch_norm_local(cocoComm *c, const ListCall &lc) {
+  static thread_local NormTable<CAP> tab;
+  const size_t es = dtype_size(lc.g_type), per = 16 / es;
+  NormArgs a = lc.norm;
+  size_t b = 0, part = 0;  // part: groups of tensor b that earlier entries hold
+  a.first = 1;
+  do {
+    int n = 0;
+    size_t at = 0;
+    while (b < lc.n && n < CAP && at < kListMaxGroups) {
+      if (lc.counts[b] == 0) {
+        ++b;
+        continue;
+      }
+      const uintptr_t p = (uintptr_t)lc.g[b];
+      const size_t head = (p & 15u) / es, len = (head + lc.counts[b] + per - 1) / per;
+      const size_t take = std::min(len - part, kListMaxGroups - at);
+      tab.g[n] = (const void *)((p & ~(uintptr_t)15u) + part * 16);
+      tab.off[n] = (unsigned)at;
+      tab.head[n] = part == 0 ? (unsigned char)head : 0;
+      tab.tail[n] = part + take == len ? (unsigned char)(len * per - head - lc.counts[b]) : 0;
+      at += take;
+      ++n;
+      part += take;
+      if (part == len) ++b, part = 0;
+    }
+    tab.off[n] = (unsigned)at;
+    while (b < lc.n && lc.counts[b] == 0) ++b;
+    a.n = n;
+    a.last = b >= lc.n;
+    const size_t units = (at + grad_norm_groups_per_warp() - 1) / grad_norm_groups_per_warp();
+    CUDA_TRY(launch_grad_norm<CAP>(lc.g_type, tab, a, c->flags, ctas_for(c, units, grad_norm_threads(), 2),
+                                   lc.stream));
+    c->launches++;
+    a.first = 0;
+  } while (!a.last);
+  return cocoSuccess;
+}
+
+int launch_list_local(cocoComm *c, const ListCall &lc) {
+  if (lc.op == kListGradNorm)
+    return lc.n <= (size_t)kNormCapSmall ? launch_norm_local<kNormCapSmall>(c, lc)
+                                         : launch_norm_local<kNormCapLarge>(c, lc);
+  return lc.n <= (size_t)kListCapSmall ? launch_adamw_local<kListCapSmall>(c, lc)
+                                       : launch_adamw_local<kListCapLarge>(c, lc);
+}
+
+// Rank `rank`'s pieces of the list.  g[b][p], out[b][p]: rank p's tensor b as
+// this rank addresses it.
+std::vector<PeerPiece> build_peer_pieces(int rank, int world, const FlatLayout &L, const ListCall &lc,
+                                         const std::vector<std::vector<char *>> &g,
+                                         const std::vector<std::vector<char *>> &out) {
+  std::vector<PeerPiece> pieces;
+  const size_t lo = std::min(L.total, (size_t)rank * L.slice), hi = std::min(L.total, lo + L.slice);
+  const size_t align = list_align(lc.op);
+  for (size_t b = 0; b < lc.n; ++b) {
+    const size_t t0 = L.off[b], t1 = t0 + lc.counts[b];
+    const size_t s0 = std::max(t0, lo), s1 = std::min(t1, hi);
+    if (s0 >= s1) continue;
+    PeerPiece pc;
+    memset(&pc, 0, sizeof(pc));
+    bool al = lc.op == kListGradNorm || aligned16(lc.w[b]);
+    for (int p = 0; p < world; ++p) {
+      pc.g[p] = g[b][p];
+      al = al && aligned16(g[b][p]);
+      if (lc.op != kListGradNorm) {
+        pc.out[p] = out[b][p];
+        al = al && aligned16(out[b][p]);
+      }
+    }
+    pc.w = lc.w ? lc.w[b] : nullptr;
+    pc.begin = s0 - t0;
+    pc.len = s1 - s0;
+    pc.off = (unsigned)((s0 - lo) / kListGroup);
+    pc.end = (unsigned)(((s1 - lo) + align - 1) / align * (align / kListGroup));
+    pc.decays = !(lc.no_decay && lc.no_decay[b]);
+    pc.aligned16 = al && pc.begin % 8 == 0 ? 1 : 0;
+    pieces.push_back(pc);
+  }
+  return pieces;
+}
+
+// The part of a PeerRank that does not depend on the piece table's address.
+PeerRank peer_rank_of(const cocoComm *c, const ListCall &lc, const FlatLayout &L, FlagPage *const flags[],
+                      const std::vector<PeerPiece> &pieces) {
+  PeerRank pr;
+  memset(&pr, 0, sizeof(pr));
+  for (int p = 0; p < c->world; ++p) pr.flags[p] = flags[p];
+  pr.n = (int)pieces.size();
+  pr.rank = c->rank;
+  pr.groups = pieces.empty() ? 0 : pieces.back().end;
+  pr.flat0 = std::min(L.total, (size_t)c->rank * L.slice);
+  pr.m = lc.adam.m, pr.v = lc.adam.v, pr.scale = lc.adam.scale;
+  pr.norm = lc.adam.norm;
+  pr.norm_out = lc.norm.out;
+  pr.state_aligned = lc.adam.state_aligned;
+  return pr;
+}
+
+// One launch for the ranks that share this device.  c: whose device memory
+// holds the tables, and whose stream order applies.
+int launch_list_peers(cocoComm *c, const ListCall &lc, std::vector<PeerRank> &ranks,
+                      const std::vector<std::vector<PeerPiece>> &pieces, size_t slice_elems,
+                      unsigned long long seq) {
+  const int nvirt = (int)ranks.size();
+  size_t bytes = sizeof(PeerRank) * nvirt;
+  for (const auto &p : pieces) bytes += sizeof(PeerPiece) * p.size();
+  if (bytes > c->list_cap) {
+    CUDA_TRY(cudaStreamSynchronize(lc.stream));
+    if (c->list_dev) CUDA_TRY(cudaFree(c->list_dev));
+    c->list_dev = nullptr;
+    c->list_cap = 0;
+    CUDA_TRY(cudaMalloc((void **)&c->list_dev, bytes * 2));
+    c->list_cap = bytes * 2;
+  }
+  std::vector<char> host(bytes);
+  size_t at = sizeof(PeerRank) * nvirt;
+  for (int k = 0; k < nvirt; ++k) {
+    ranks[k].pieces = (const PeerPiece *)(c->list_dev + at);
+    if (!pieces[k].empty()) memcpy(host.data() + at, pieces[k].data(), sizeof(PeerPiece) * pieces[k].size());
+    at += sizeof(PeerPiece) * pieces[k].size();
+  }
+  memcpy(host.data(), ranks.data(), sizeof(PeerRank) * nvirt);
+  // pageable source: staged before the call returns; ordered on the stream
+  // after the previous call's kernel, which may still be reading the table
+  CUDA_TRY(cudaMemcpyAsync(c->list_dev, host.data(), bytes, cudaMemcpyHostToDevice, lc.stream));
+  PeerArgs pa = {};
+  pa.ranks = (const PeerRank *)c->list_dev;
+  pa.world = c->world;
+  pa.seq = seq;
+  pa.timeout_ns = (unsigned long long)c->timeout_ms * 1000000ull;
+  ListLaunch cfg = {};
+  const bool norm = lc.op == kListGradNorm, quant = lc.op == kListAdamWQuant;
+  cfg.threads = norm ? grad_norm_threads() : 256;
+  cfg.nvirt = nvirt;
+  cfg.cooperative = nvirt > 1;
+  if (cfg.cooperative && !c->coop_supported) return cocoInvalidUsage;
+  int occ = 0;
+  CUDA_TRY(norm ? grad_norm_peers_occupancy(lc.g_type, c->world, cfg.threads, &occ)
+                : adamw_peers_occupancy(quant, lc.g_type, c->world, cfg.threads, &occ));
+  if (occ < 1) return cocoInternalError;
+  cfg.ctas = ctas_for(c, (slice_elems + kListUnit - 1) / kListUnit, cfg.threads, occ);
+  if (nvirt > 1)  // all ranks' CTAs have to be resident at once
+    cfg.ctas = std::max(1, std::min(cfg.ctas, occ * c->sm_count / nvirt));
+  CUDA_TRY(norm ? launch_grad_norm_peers(lc.g_type, pa, lc.norm, cfg, lc.stream)
+                : launch_adamw_peers(quant, lc.g_type, pa, lc.adam, cfg, lc.stream));
+  c->launches++;
+  return cocoSuccess;
+}
+
+// Every rank of a single-process group has called.
+int flush_list_group(LocalGroup *grp) {
+  const int R = (int)grp->comms.size();
+  const ListCall &first = grp->comms[0]->pending.list->call;
+  const unsigned long long seq = grp->comms[0]->pending.sa.seq;
+  FlagPage *flags[kMaxRanks];
+  std::vector<std::vector<char *>> g(first.n), out(first.n);
+  for (size_t b = 0; b < first.n; ++b) g[b].resize(R), out[b].resize(R);
+  for (int r = 0; r < R; ++r) {
+    const PendingCall &pc = grp->comms[r]->pending;
+    const ListCall &lc = pc.list->call;
+    if (lc.op != first.op || lc.n != first.n || lc.g_type != first.g_type || (lc.lp != nullptr) != (first.lp != nullptr) ||
+        lc.lp_type != first.lp_type || pc.sa.seq != seq ||
+        memcmp(lc.counts, first.counts, sizeof(size_t) * first.n) != 0)
+      return cocoInvalidUsage;  // ranks disagree on the operation
+    flags[r] = grp->comms[r]->flags;
+    for (size_t b = 0; b < first.n; ++b) {
+      g[b][r] = (char *)lc.g[b];
+      out[b][r] = lc.lp ? (char *)lc.lp[b] : lc.w ? (char *)lc.w[b] : nullptr;
+    }
+  }
+  const FlatLayout L = flat_layout(first.counts, first.n, R, list_align(first.op));
+  std::map<int, std::vector<cocoComm *>> by_dev;
+  for (cocoComm *c : grp->comms) by_dev[c->device].push_back(c);
+  for (auto &kv : by_dev) {
+    DeviceGuard guard(kv.first);
+    if (!guard.ok) return cocoCudaError;
+    std::vector<PeerRank> ranks;
+    std::vector<std::vector<PeerPiece>> pieces;
+    for (cocoComm *c : kv.second) {
+      const ListCall &lc = c->pending.list->call;
+      pieces.push_back(build_peer_pieces(c->rank, R, L, lc, g, out));
+      ranks.push_back(peer_rank_of(c, lc, L, flags, pieces.back()));
+    }
+    COCO_TRY(launch_list_peers(kv.second[0], kv.second[0]->pending.list->call, ranks, pieces, L.slice, seq));
+  }
+  return cocoSuccess;
+}
+
+// Checks that need no device; `total`: elements of the list.
+int validate_list(const cocoComm *c, const ListCall &lc, size_t *total) {
+  const size_t es = dtype_size(lc.g_type);
+  if (es == 0) return cocoInvalidArgument;
+  const bool adam = lc.op != kListGradNorm, quant = lc.op == kListAdamWQuant;
+  if (lc.lp && lc.lp_type != cocoFloat16 && lc.lp_type != cocoBfloat16) return cocoInvalidArgument;
+  *total = 0;
+  for (size_t b = 0; b < lc.n; ++b) {
+    const size_t count = lc.counts[b];
+    if (count == 0) continue;  // an empty tensor's pointers are not looked at
+    if (count > kListMaxGroups * kListGroup || !lc.g[b] || (uintptr_t)lc.g[b] % es) return cocoInvalidArgument;
+    if (adam && (!lc.w[b] || (uintptr_t)lc.w[b] % 4)) return cocoInvalidArgument;
+    if (lc.lp && (!lc.lp[b] || (uintptr_t)lc.lp[b] % 2)) return cocoInvalidArgument;
+    *total += count;
+  }
+  if (c->world > 1 &&
+      flat_layout(lc.counts, lc.n, c->world, list_align(lc.op)).slice > kListMaxGroups * kListGroup)
+    return cocoInvalidArgument;
+  if (adam) {
+    const AdamWArgs &a = lc.adam;
+    if ((uintptr_t)a.norm % 4) return cocoInvalidArgument;
+    if (*total > 0) {
+      if (!a.m || !a.v || (quant && !a.scale)) return cocoInvalidArgument;
+      if (quant ? (uintptr_t)a.scale % 2 : ((uintptr_t)a.m % 4 || (uintptr_t)a.v % 4)) return cocoInvalidArgument;
+    }
+  }
+  return cocoSuccess;
+}
+
+int enqueue_list_or_throw(cocoComm *c, ListCall &lc) {
+  size_t total = 0;
+  COCO_TRY(validate_list(c, lc, &total));
+  if (total == 0 && lc.op != kListGradNorm) return cocoSuccess;
+  if (lc.op != kListGradNorm) {
+    const uintptr_t mask = lc.op == kListAdamWQuant ? 3u : 15u;
+    lc.adam.state_aligned = (((uintptr_t)lc.adam.m | (uintptr_t)lc.adam.v) & mask) == 0;
+    lc.adam.lp_kind = !lc.lp ? kLpNone : lc.lp_type == cocoFloat16 ? kLpF16 : kLpBf16;
+  }
+  NvtxRange range(lc.op == kListGradNorm ? "coconet gradient norm" : "coconet fused AdamW");
+  if (c->group) {  // single-process ranks: wait until every one of them has called
+    if (c->has_pending) return cocoInvalidUsage;
+    COCO_TRY(refuse_capture(c, lc.stream));
+    c->pending = PendingCall();
+    c->pending.list = std::make_shared<OwnedListCall>(lc);
+    c->pending.sa.seq = ++c->seq;
+    c->has_pending = true;
+    if (g_group_depth > 0) {
+      if (std::find(g_group_touched.begin(), g_group_touched.end(), c) == g_group_touched.end())
+        g_group_touched.push_back(c);
+      return cocoSuccess;
+    }
+    for (cocoComm *o : c->group->comms)
+      if (!o->has_pending) return cocoSuccess;  // more ranks to come
+    return flush_group(c->group.get());
+  }
+  DeviceGuard guard(c->device);
+  if (!guard.ok) return cocoCudaError;
+  if (c->world == 1) return launch_list_local(c, lc);
+  COCO_TRY(refuse_capture(c, lc.stream));
+  const unsigned long long seq = ++c->seq;
+  std::vector<std::vector<char *>> g(lc.n), out(lc.n);
+  for (size_t b = 0; b < lc.n; ++b) {
+    g[b].resize(kMaxRanks), out[b].resize(kMaxRanks);
+    if (lc.counts[b] == 0) continue;
+    char *mc = nullptr;
+    COCO_TRY(peer_views(c, lc.g[b], lc.counts[b] * dtype_size(lc.g_type), g[b].data(), &mc));
+    if (lc.lp)
+      COCO_TRY(peer_views(c, lc.lp[b], lc.counts[b] * 2, out[b].data(), &mc));
+    else if (lc.w)
+      COCO_TRY(peer_views(c, lc.w[b], lc.counts[b] * sizeof(float), out[b].data(), &mc));
+  }
+  const FlatLayout L = flat_layout(lc.counts, lc.n, c->world, list_align(lc.op));
+  const std::vector<std::vector<PeerPiece>> pieces = {build_peer_pieces(c->rank, c->world, L, lc, g, out)};
+  std::vector<PeerRank> ranks = {peer_rank_of(c, lc, L, c->peer_flags, pieces[0])};
+  return launch_list_peers(c, lc, ranks, pieces, L.slice, seq);
+}
+
+// No exception (the host ran out of memory) leaves a C entry point.
+int enqueue_list(cocoComm *c, ListCall &lc) {
+  try {
+    return enqueue_list_or_throw(c, lc);
+  } catch (...) {
+    return cocoInternalError;
+  }
+}
 
 int enqueue(cocoComm *c, PendingCall &pc) {
   NvtxRange range(pc);
@@ -1135,6 +1529,7 @@ int cocoCommDestroy(cocoComm_t comm) {
         cudaFree(kv.second);
       }
   }
+  if (comm->list_dev) cudaFree(comm->list_dev);
   if (comm->seg_part) cudaFree(comm->seg_part);
   if (comm->flags) cudaFree(comm->flags);
   if (comm->seg_dev) cudaFree(comm->seg_dev);
@@ -1510,6 +1905,105 @@ int cocoFusedLAMBScattered(cocoComm_t comm, size_t nbuff, const void *const *g,
   pc.sa.flags = flags;
   set_denominators(&pc.sa, kLAMB, step);
   return enqueue_scattered(comm, kLAMB, nbuff, g, g_type, w, counts, m, v, pc, stream);
+}
+
+int cocoQuantSliceElems(size_t nbuff, const size_t *counts, int world, size_t *slice_elems) {
+  if (!counts || !slice_elems || world < 1 || world > kMaxRanks) return cocoInvalidArgument;
+  try {
+    *slice_elems = flat_layout(counts, nbuff, world, kListUnit).slice;
+  } catch (...) {
+    return cocoInternalError;
+  }
+  return cocoSuccess;
+}
+
+int cocoQuantTensorPlace(size_t nbuff, const size_t *counts, int world, size_t tensor,
+                         size_t *flat_offset, int *first_rank, int *last_rank) {
+  if (!counts || !flat_offset || !first_rank || !last_rank || world < 1 || world > kMaxRanks ||
+      tensor >= nbuff)
+    return cocoInvalidArgument;
+  try {
+    const FlatLayout L = flat_layout(counts, nbuff, world, kListUnit);
+    *flat_offset = L.off[tensor];
+    if (counts[tensor] == 0) {
+      *first_rank = *last_rank = -1;
+    } else {  // the same arithmetic as build_peer_pieces
+      *first_rank = (int)(L.off[tensor] / L.slice);
+      *last_rank = (int)((L.off[tensor] + counts[tensor] - 1) / L.slice);
+    }
+  } catch (...) {
+    return cocoInternalError;
+  }
+  return cocoSuccess;
+}
+
+int cocoGradNormScattered(cocoComm_t comm, size_t nbuff, const void *const *g, cocoDataType_t g_type,
+                          const size_t *counts, float grad_scale, float max_norm, float *norm,
+                          cocoStream_t stream) {
+  if (!comm || nbuff == 0 || !g || !counts || !norm || (uintptr_t)norm % 4) return cocoInvalidArgument;
+  if (!std::isfinite(grad_scale) || std::isnan(max_norm)) return cocoInvalidArgument;
+  ListCall lc;
+  lc.op = kListGradNorm;
+  lc.n = nbuff, lc.g = g, lc.g_type = g_type, lc.counts = counts;
+  lc.norm.out = norm;
+  lc.norm.scale = std::fabs((double)grad_scale);
+  lc.norm.max_norm = max_norm;
+  lc.stream = (cudaStream_t)stream;
+  return enqueue_list(comm, lc);
+}
+
+// What the two AdamW forms share: checks and the step's scalars.
+static int adamw_call(ListCall *lc, cocoComm_t comm, size_t nbuff, const void *const *g, cocoDataType_t g_type,
+                      float *const *w, void *const *w_lp, cocoDataType_t lp_type, const size_t *counts,
+                      void *m, void *v, float lr, float beta1, float beta2, float eps, float weight_decay,
+                      const unsigned char *no_decay, int step, float grad_scale, const float *norm,
+                      cocoStream_t stream) {
+  if (!comm || nbuff == 0 || !g || !w || !counts || step < 0) return cocoInvalidArgument;
+  if (!(beta1 >= 0.f && beta1 < 1.f && beta2 >= 0.f && beta2 < 1.f && eps >= 0.f)) return cocoInvalidArgument;
+  if (!std::isfinite(lr) || !std::isfinite(weight_decay) || !std::isfinite(eps) || !std::isfinite(grad_scale))
+    return cocoInvalidArgument;
+  lc->n = nbuff, lc->g = g, lc->g_type = g_type, lc->w = w, lc->lp = w_lp, lc->lp_type = lp_type;
+  lc->counts = counts, lc->no_decay = no_decay;
+  AdamWArgs &a = lc->adam;
+  a.m = m, a.v = v, a.norm = norm;
+  const double t = (double)step + 1.0;
+  const double d1 = 1.0 - std::pow((double)beta1, t), d2 = 1.0 - std::pow((double)beta2, t);
+  a.grad_scale = grad_scale, a.beta1 = beta1, a.beta2 = beta2;
+  a.omb1 = 1.0f - beta1, a.omb2 = 1.0f - beta2;
+  a.c1 = (float)((double)lr / d1);
+  a.rs2 = (float)(1.0 / std::sqrt(d2));
+  a.eps = eps;
+  a.decay = (float)(1.0 - (double)lr * (double)weight_decay);
+  lc->stream = (cudaStream_t)stream;
+  return cocoSuccess;
+}
+
+int cocoFusedAdamWScattered(cocoComm_t comm, size_t nbuff, const void *const *g, cocoDataType_t g_type,
+                            float *const *w, void *const *w_lp, cocoDataType_t lp_type,
+                            const size_t *counts, float *m, float *v, float lr, float beta1,
+                            float beta2, float eps, float weight_decay, const unsigned char *no_decay,
+                            int step, float grad_scale, const float *norm, cocoStream_t stream) {
+  ListCall lc;
+  lc.op = kListAdamW;
+  COCO_TRY(adamw_call(&lc, comm, nbuff, g, g_type, w, w_lp, lp_type, counts, m, v, lr, beta1, beta2, eps,
+                      weight_decay, no_decay, step, grad_scale, norm, stream));
+  return enqueue_list(comm, lc);
+}
+
+int cocoFusedAdamWQuantScattered(cocoComm_t comm, size_t nbuff, const void *const *g,
+                                 cocoDataType_t g_type, float *const *w, void *const *w_lp,
+                                 cocoDataType_t lp_type, const size_t *counts, unsigned char *m,
+                                 unsigned char *vroot, unsigned char *scale, float lr, float beta1,
+                                 float beta2, float eps, float weight_decay,
+                                 const unsigned char *no_decay, int step, uint64_t seed,
+                                 float grad_scale, const float *norm, cocoStream_t stream) {
+  ListCall lc;
+  lc.op = kListAdamWQuant;
+  COCO_TRY(adamw_call(&lc, comm, nbuff, g, g_type, w, w_lp, lp_type, counts, m, vroot, lr, beta1, beta2, eps,
+                      weight_decay, no_decay, step, grad_scale, norm, stream));
+  lc.adam.scale = scale;
+  lc.adam.key = adamw_rounding_key(seed, step);
+  return enqueue_list(comm, lc);
 }
 
 int cocoLinkProbe(cocoComm_t comm, void *buf, size_t bytes, int mode, int unroll, int iters,

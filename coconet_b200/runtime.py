@@ -10,6 +10,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 
 VARIANT_OVERLAP, VARIANT_DSL, VARIANT_NCCL = 0, 1, 2
 LAMB_REF_QUIRK = 0x1
+QUANT_BLOCK = 256
 _F16, _F32, _BF16 = 6, 7, 9
 
 
@@ -96,6 +97,26 @@ _SIGNATURES = {
                                          C.c_void_p, C.c_float, C.c_float, C.c_float, C.c_float,
                                          C.c_float, C.c_int, C.c_float, C.c_int, C.c_uint,
                                          C.c_void_p]),
+    "cocoGradNormScattered": (C.c_int, [C.c_void_p, C.c_size_t, C.POINTER(C.c_void_p), C.c_int,
+                                        C.POINTER(C.c_size_t), C.c_float, C.c_float, C.c_void_p,
+                                        C.c_void_p]),
+    "cocoFusedAdamWScattered": (C.c_int, [C.c_void_p, C.c_size_t, C.POINTER(C.c_void_p), C.c_int,
+                                          C.POINTER(C.c_void_p), C.POINTER(C.c_void_p), C.c_int,
+                                          C.POINTER(C.c_size_t), C.c_void_p, C.c_void_p, C.c_float,
+                                          C.c_float, C.c_float, C.c_float, C.c_float,
+                                          C.POINTER(C.c_ubyte), C.c_int, C.c_float, C.c_void_p,
+                                          C.c_void_p]),
+    "cocoFusedAdamWQuantScattered": (C.c_int, [C.c_void_p, C.c_size_t, C.POINTER(C.c_void_p), C.c_int,
+                                               C.POINTER(C.c_void_p), C.POINTER(C.c_void_p), C.c_int,
+                                               C.POINTER(C.c_size_t), C.c_void_p, C.c_void_p,
+                                               C.c_void_p, C.c_float, C.c_float, C.c_float, C.c_float,
+                                               C.c_float, C.POINTER(C.c_ubyte), C.c_int, C.c_uint64,
+                                               C.c_float, C.c_void_p, C.c_void_p]),
+    "cocoQuantSliceElems": (C.c_int, [C.c_size_t, C.POINTER(C.c_size_t), C.c_int,
+                                      C.POINTER(C.c_size_t)]),
+    "cocoQuantTensorPlace": (C.c_int, [C.c_size_t, C.POINTER(C.c_size_t), C.c_int, C.c_size_t,
+                                       C.POINTER(C.c_size_t), C.POINTER(C.c_int),
+                                       C.POINTER(C.c_int)]),
     "cocoAllReduce": (C.c_int, [C.c_void_p, C.c_void_p, C.c_size_t, C.c_void_p]),
     "cocoReduceScatter": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_size_t, C.c_void_p]),
     "cocoAllGather": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_size_t, C.c_void_p]),
@@ -160,6 +181,43 @@ def scattered_slice_elems(counts, world):
     out = C.c_size_t()
     _check(lib().cocoScatteredSliceElems(len(counts), arr, world, C.byref(out)), "cocoScatteredSliceElems")
     return out.value
+
+
+def quant_tensor_place(counts, world, tensor):
+    """scattered_tensor_place for the 8-bit moments of fused_adamw_quant_scattered."""
+    arr = (C.c_size_t * len(counts))(*counts)
+    off, r0, r1 = C.c_size_t(), C.c_int(), C.c_int()
+    _check(lib().cocoQuantTensorPlace(len(counts), arr, world, tensor, C.byref(off),
+                                      C.byref(r0), C.byref(r1)), "cocoQuantTensorPlace")
+    return off.value, r0.value, r1.value
+
+
+def quant_slice_elems(counts, world):
+    """Elements of 8-bit m / vroot each rank holds for a list of tensors of these
+    sizes (a multiple of QUANT_BLOCK; one pair of scale bytes per block)."""
+    arr = (C.c_size_t * len(counts))(*counts)
+    out = C.c_size_t()
+    _check(lib().cocoQuantSliceElems(len(counts), arr, world, C.byref(out)), "cocoQuantSliceElems")
+    return out.value
+
+
+def quant_state(counts, world, device=None):
+    """(m, vroot, scale) of fused_adamw_quant_scattered before the first step, for
+    one rank: e4m3 codes, and per block the e8m0 scales of m and of vroot."""
+    import torch
+    n = quant_slice_elems(counts, world)
+    zeros = [torch.zeros(k, dtype=torch.uint8, device=device or "cuda") for k in (n, n, n // QUANT_BLOCK * 2)]
+    return (zeros[0].view(torch.float8_e4m3fn), zeros[1].view(torch.float8_e4m3fn),
+            zeros[2].view(torch.float8_e8m0fnu).view(-1, 2))
+
+
+def quant_decode(m, vroot, scale):
+    """The fp32 moments (m, v) that an 8-bit state stands for."""
+    import torch
+    s = scale.reshape(-1).view(torch.float8_e8m0fnu).float().view(-1, 2)
+    a = m.view(torch.float8_e4m3fn).float().view(-1, QUANT_BLOCK) * s[:, 0:1]
+    b = vroot.view(torch.float8_e4m3fn).float().view(-1, QUANT_BLOCK) * s[:, 1:2]
+    return a.view(-1), (b * b).view(-1)
 
 
 def topology_check(world, access, perf_rank):
@@ -252,14 +310,62 @@ class TensorList:
     methods; converting a few hundred tensors on every call costs more host
     time than the step takes on the device."""
 
-    def __init__(self, gs, ws):
-        assert len(gs) == len(ws) and len(gs) > 0
-        self.tensors = (list(gs), list(ws))   # keeps the memory alive
+    def __init__(self, gs, ws, lps=None, no_decay=None):
+        """`ws` may be None for a list that only the gradient norm reads.  `lps`:
+        16-bit copies of the weights, `no_decay`: a truth value per tensor (the
+        AdamW calls read both)."""
+        assert len(gs) > 0 and (ws is None or len(gs) == len(ws))
+        if lps is not None and (ws is None or len(lps) != len(gs)):
+            raise ValueError("one low-precision copy per weight tensor is needed")
+        if no_decay is not None and len(no_decay) != len(gs):
+            raise ValueError("no_decay holds one value per tensor")
+        self.tensors = (list(gs), list(ws) if ws is not None else None,
+                        list(lps) if lps is not None else None)   # keeps the memory alive
         self.n = len(gs)
         self.g = (C.c_void_p * self.n)(*[t.data_ptr() for t in gs])
-        self.w = (C.c_void_p * self.n)(*[t.data_ptr() for t in ws])
-        self.counts = (C.c_size_t * self.n)(*[t.numel() for t in ws])
+        self.w = (C.c_void_p * self.n)(*[t.data_ptr() for t in ws]) if ws is not None else None
+        self.counts = (C.c_size_t * self.n)(*[t.numel() for t in (gs if ws is None else ws)])
         self.dtype = _dtype_code(gs[0])
+        self.lp = (C.c_void_p * self.n)(*[t.data_ptr() for t in lps]) if lps is not None else None
+        self.lp_dtype = _dtype_code(lps[0]) if lps is not None else _F16
+        self.no_decay = (C.c_ubyte * self.n)(*[1 if x else 0 for x in no_decay]) if no_decay is not None else None
+        self._device = None   # set once the list has passed _checked
+        self._slices = {}
+
+    def _checked(self, weights):
+        """Types, sizes and devices of the list, looked over at its first use by
+        the gradient norm or an AdamW call.  Returns the device."""
+        gs, ws, lps = self.tensors
+        if weights and ws is None:
+            raise ValueError("this list holds no weights")
+        if self._device is None:
+            import torch
+            dev = gs[0].device
+            index = gs[0].get_device() if gs[0].is_cuda else None
+            for what, ts, like in (("gradient", gs, gs[0].dtype), ("weight", ws, torch.float32),
+                                   ("low-precision copy", lps, lps[0].dtype if lps else None)):
+                for k, (t, count) in enumerate(zip(ts or (), self.counts)):
+                    if t.dtype != like:
+                        raise ValueError(f"{what} {k} is {t.dtype}, not {like}")
+                    if t.get_device() != index:
+                        raise ValueError(f"{what} {k} is on {t.device}; one CUDA device is needed ({dev})")
+                    if not t.is_contiguous():
+                        raise ValueError(f"{what} {k} is not contiguous")
+                    if t.numel() != count:
+                        raise ValueError(f"{what} {k} holds {t.numel()} elements, not {count}")
+            if lps and lps[0].dtype not in (torch.float16, torch.bfloat16):
+                raise ValueError(f"low-precision copies are fp16 or bf16, not {lps[0].dtype}")
+            self._device = dev
+        return self._device
+
+    def _slice(self, world, quant):
+        key = (world, quant)
+        if key not in self._slices:
+            out = C.c_size_t()
+            fn = lib().cocoQuantSliceElems if quant else lib().cocoScatteredSliceElems
+            _check(fn(self.n, self.counts, world, C.byref(out)), "slice of a list")
+            self._slices[key] = out.value
+        return self._slices[key]
 
 
 def _list_dtype(gs):
@@ -428,6 +534,73 @@ class Communicator:
                                             _ptr(v), lr, beta1, beta2, eps, weight_decay, step,
                                             grad_scale, variant, flags, _stream(stream)),
                "cocoFusedLAMBScattered")
+
+    # ---- AdamW and the gradient norm over a list ----
+    def _on(self, device, stream):
+        """The stream to use: `stream`, or the current one of the list's device,
+        which has to be this communicator's."""
+        import torch
+        if getattr(self, "_device", None) is None:
+            d = C.c_int()
+            _check(lib().cocoCommCuDevice(self._h, C.byref(d)), "cocoCommCuDevice")
+            self._device = d.value
+        if device.index != self._device:
+            raise ValueError(f"the tensors are on {device}, the communicator on cuda:{self._device}")
+        return C.c_void_p((stream if stream is not None else torch.cuda.current_stream(device)).cuda_stream)
+
+    @staticmethod
+    def _held(t, what, device, dtypes, least):
+        """Pointer of a state tensor after a look at its type and size."""
+        if t.dtype not in dtypes or t.device != device or not t.is_contiguous() or t.numel() < least:
+            raise ValueError(f"{what}: at least {least} contiguous elements of {' or '.join(map(str, dtypes))} on "
+                             f"{device} are needed, got {tuple(t.shape)} {t.dtype} on {t.device}")
+        return t.data_ptr()
+
+    def grad_norm_scattered(self, gs, norm, max_norm=0.0, grad_scale=1.0, stream=None):
+        """norm[0] = |grad_scale| * the 2-norm of the summed gradients of the list,
+        norm[1] = the factor that clips it to max_norm (<= 0: 1).  `norm`: two
+        fp32 on the device; pass it to the AdamW calls."""
+        import torch
+        lst = gs if isinstance(gs, TensorList) else TensorList(gs, None)
+        device = lst._checked(weights=False)
+        p = self._held(norm, "norm", device, (torch.float32,), 2)
+        _check(lib().cocoGradNormScattered(self._h, lst.n, lst.g, lst.dtype, lst.counts, grad_scale,
+                                           max_norm, p, self._on(device, stream)),
+               "cocoGradNormScattered")
+
+    def fused_adamw_scattered(self, gs, ws, m, v, lr, beta1, beta2, eps, weight_decay, step,
+                              w_lps=None, no_decay=None, grad_scale=1.0, norm=None, stream=None):
+        """AdamW over a list, fp32 moments.  `norm`: as grad_norm_scattered left it;
+        the gradients are scaled by norm[1], and a norm that is not finite skips
+        the step.  With a TensorList, its copies and no_decay apply."""
+        import torch
+        lst = gs if isinstance(gs, TensorList) else TensorList(gs, ws, w_lps, no_decay)
+        device = lst._checked(weights=True)
+        need, f32 = lst._slice(self.world, False), (torch.float32,)
+        _check(lib().cocoFusedAdamWScattered(
+            self._h, lst.n, lst.g, lst.dtype, lst.w, lst.lp, lst.lp_dtype, lst.counts,
+            self._held(m, "m", device, f32, need), self._held(v, "v", device, f32, need),
+            lr, beta1, beta2, eps, weight_decay, lst.no_decay, step, grad_scale,
+            self._held(norm, "norm", device, f32, 2) if norm is not None else None,
+            self._on(device, stream)), "cocoFusedAdamWScattered")
+
+    def fused_adamw_quant_scattered(self, gs, ws, m, vroot, scale, lr, beta1, beta2, eps, weight_decay,
+                                    step, seed, w_lps=None, no_decay=None, grad_scale=1.0, norm=None,
+                                    stream=None):
+        """AdamW over a list with 8-bit moments (see quant_state): e4m3 codes of m
+        and sqrt(v), rounded at random from `seed` and `step`."""
+        import torch
+        lst = gs if isinstance(gs, TensorList) else TensorList(gs, ws, w_lps, no_decay)
+        device = lst._checked(weights=True)
+        need = lst._slice(self.world, True)
+        code, exponent = (torch.float8_e4m3fn, torch.uint8), (torch.float8_e8m0fnu, torch.uint8)
+        _check(lib().cocoFusedAdamWQuantScattered(
+            self._h, lst.n, lst.g, lst.dtype, lst.w, lst.lp, lst.lp_dtype, lst.counts,
+            self._held(m, "m", device, code, need), self._held(vroot, "vroot", device, code, need),
+            self._held(scale, "scale", device, exponent, need // QUANT_BLOCK * 2),
+            lr, beta1, beta2, eps, weight_decay, lst.no_decay, step, seed, grad_scale,
+            self._held(norm, "norm", device, (torch.float32,), 2) if norm is not None else None,
+            self._on(device, stream)), "cocoFusedAdamWQuantScattered")
 
     def link_probe(self, buf, mode, unroll=1, iters=5, stream=None):
         """GB/s per direction per GPU of a pull ("pull"), push ("push"), pull +

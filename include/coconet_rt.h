@@ -54,6 +54,7 @@ extern "C" {
 #define COCO_VERSION 100
 #define COCO_MAX_RANKS 8
 #define COCO_MAX_LAMB_TENSORS 2048 /* tensors of one cocoFusedLAMBScattered call */
+#define COCO_QUANT_BLOCK 256       /* elements of 8-bit moments that share a scale */
 
 typedef struct cocoComm *cocoComm_t;
 
@@ -327,6 +328,75 @@ int cocoFusedLAMBScattered(cocoComm_t comm, size_t nbuff, const void *const *g,
                            float *v, float lr, float beta1, float beta2, float eps,
                            float weight_decay, int step, float grad_scale, cocoVariant_t variant,
                            unsigned flags, cocoStream_t stream);
+/* ---- AdamW and the gradient norm over a list of tensors -----------------------
+ * The update of a transformer's training step: clip by the global norm, decay
+ * the weights apart from the gradient, keep the moments in fp32 or in 8 bits.
+ * Lists, slices and the order of the ranks' sums are those of the scattered
+ * calls above; world sizes 1..COCO_MAX_RANKS, peer-to-peer path.  No reference
+ * counterpart: its Adam has no decay and no list has low-precision copies.
+ *  - A tensor of 0 elements is allowed and its pointers are not looked at.
+ *    Gradients, weights, copies and state must not overlap one another.
+ *  - Elements need only the alignment of their type; tensors that start on 16
+ *    bytes are faster.
+ *  - World size 1: a call is one kernel per 1024 tensors and keeps nothing of the
+ *    list, so it may be captured into a CUDA graph; the scalars are replayed as
+ *    they were captured.  Above it a call that is being captured is refused
+ *    (cocoInvalidUsage).
+ *
+ * cocoGradNormScattered:  norm[0] = |grad_scale| * || sum over ranks of g ||_2
+ * over the whole list, norm[1] = max_norm / norm[0] where 0 < max_norm < norm[0]
+ * and 1 elsewhere (max_norm <= 0: never clip), 0 where norm[0] is inf or nan.
+ * `norm`: two fp32 in this GPU's memory, the same values on every rank.  The sum
+ * is held in fp64 and its order is fixed per launch shape, so repeated calls
+ * agree to the last bit.
+ *
+ * cocoFusedAdamWScattered, with d1 = 1 - beta1^(step+1), d2 = 1 - beta2^(step+1):
+ *     g <- (sum over ranks of g) * (norm ? norm[1] * grad_scale : grad_scale)
+ *     m <- beta1 m + (1 - beta1) g        v <- beta2 v + (1 - beta2) g^2
+ *     w <- w (1 - lr weight_decay) - (lr / d1) m / (sqrt(v) / sqrt(d2) + eps)
+ * every operation rounded to fp32.  With `norm` (as cocoGradNormScattered left it
+ * on every rank) whose norm[0] is inf or nan the step changes nothing.
+ *   w_lp      NULL, or per tensor a 16-bit copy of w (lp_type), gathered instead
+ *             of w; then, as in the flat call, only the own slice of w is updated
+ *   no_decay  NULL, or per tensor a byte (host): not 0 = weight_decay does not apply
+ *   m, v      as in cocoFusedAdamScattered (cocoScatteredSliceElems elements), and
+ *             interchangeable with its moments
+ * 0 <= beta < 1, eps >= 0, step >= 0, all finite, else cocoInvalidArgument.
+ *
+ * cocoFusedAdamWQuantScattered: the same step with the moments in 8 bits: m and
+ * vroot = sqrt(v) as e4m3 codes (one byte per element), and per COCO_QUANT_BLOCK
+ * elements two e8m0 scale bytes {of m, of vroot} in `scale`; an element's value is
+ * code * 2^(scale byte - 127).  In the flat layout of this state every tensor
+ * starts at a multiple of COCO_QUANT_BLOCK elements and so does every slice:
+ * cocoQuantSliceElems bytes of m and of vroot per rank, and that / 128 bytes of
+ * scale.  Bytes that belong to no element are left alone.  All bytes 0 is the
+ * state before the first step.  The weights are updated from the new moments in
+ * fp32, before they are rounded.  Codes are rounded up or down at random, up with
+ * the probability of the part cut off (to nearest, a beta2 of 0.999 would never
+ * move vroot); the random bits are a function of `seed`, `step` and the element's
+ * place in the flat state, so that a step is reproducible, and the same at every
+ * world size.  A vroot above 0 is never stored as 0; a block in which a moment is
+ * inf or nan gets scale byte 255, which reads back as nan. */
+int cocoGradNormScattered(cocoComm_t comm, size_t nbuff, const void *const *g,
+                          cocoDataType_t g_type, const size_t *counts, float grad_scale,
+                          float max_norm, float *norm, cocoStream_t stream);
+int cocoFusedAdamWScattered(cocoComm_t comm, size_t nbuff, const void *const *g,
+                            cocoDataType_t g_type, float *const *w, void *const *w_lp,
+                            cocoDataType_t lp_type, const size_t *counts, float *m, float *v,
+                            float lr, float beta1, float beta2, float eps, float weight_decay,
+                            const unsigned char *no_decay, int step, float grad_scale,
+                            const float *norm, cocoStream_t stream);
+int cocoFusedAdamWQuantScattered(cocoComm_t comm, size_t nbuff, const void *const *g,
+                                 cocoDataType_t g_type, float *const *w, void *const *w_lp,
+                                 cocoDataType_t lp_type, const size_t *counts, unsigned char *m,
+                                 unsigned char *vroot, unsigned char *scale, float lr, float beta1,
+                                 float beta2, float eps, float weight_decay,
+                                 const unsigned char *no_decay, int step, uint64_t seed,
+                                 float grad_scale, const float *norm, cocoStream_t stream);
+/* cocoScatteredSliceElems and cocoScatteredTensorPlace for the 8-bit state. */
+int cocoQuantSliceElems(size_t nbuff, const size_t *counts, int world, size_t *slice_elems);
+int cocoQuantTensorPlace(size_t nbuff, const size_t *counts, int world, size_t tensor,
+                         size_t *flat_offset, int *first_rank, int *last_rank);
 
 /* ---- stand-alone collectives (fp32, sum) ------------------------------------
  * What the unfused schedules of a generated program call where the reference
