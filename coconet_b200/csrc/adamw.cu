@@ -4,8 +4,8 @@
 //   g <- (sum over ranks of g) * grad_scale * clip
 //   m <- beta1 m + (1 - beta1) g        v <- beta2 v + (1 - beta2) g^2
 //   w <- w (1 - lr decay) - (lr / d1) m / (sqrt(v) / sqrt(d2) + eps)
-// Every operation is rounded to fp32 by itself, so the results do not depend on
-// the path an element takes and match a scalar evaluation bit for bit.
+// All paths run the same roundings, so the results do not depend on the path an
+// element takes; moments, codes and scales match a scalar evaluation bit for bit.
 //
 // 8-bit moments: m and r = sqrt(v) as e4m3 codes with one power-of-two scale
 // per 256 elements (e8m0: the exponent byte of a float).  r and not v: the
@@ -45,11 +45,14 @@ template <> struct View<1> {
 
 template <int RB> __device__ __forceinline__ void put_lp4(const View<RB> &v, int R, int kind, size_t i,
                                                           const float (&x)[4]) {
-  unsigned short h[4];
-#pragma unroll
-  for (int e = 0; e < 4; ++e)
-    h[e] = kind == kLpF16 ? Bits16<__half>::from_f32(x[e]) : Bits16<__nv_bfloat16>::from_f32(x[e]);
-  const uint2 q = make_uint2(h[0] | ((unsigned)h[1] << 16), h[2] | ((unsigned)h[3] << 16));
+  uint2 q;
+  if (kind == kLpF16) {
+    const __half2 a = __floats2half2_rn(x[0], x[1]), b = __floats2half2_rn(x[2], x[3]);
+    q = make_uint2(*reinterpret_cast<const unsigned *>(&a), *reinterpret_cast<const unsigned *>(&b));
+  } else {
+    const __nv_bfloat162 a = __floats2bfloat162_rn(x[0], x[1]), b = __floats2bfloat162_rn(x[2], x[3]);
+    q = make_uint2(*reinterpret_cast<const unsigned *>(&a), *reinterpret_cast<const unsigned *>(&b));
+  }
   if constexpr (RB == 1) {
     *reinterpret_cast<uint2 *>((unsigned short *)v.lp + i) = q;
   } else {
@@ -95,48 +98,121 @@ template <int RB> __device__ __forceinline__ void put_w1(const View<RB> &v, int 
 }
 
 // ---- the update ------------------------------------------------------------------
-__device__ __forceinline__ void moments(const AdamWArgs &a, float g, float &m, float &v) {
+// The reciprocal is the hardware's, within 2^-23, and so is the root of fp32
+// moments: the exact ones branch per element, which keeps the elements' chains
+// from overlapping (104 us against 74 for 12.6 M elements), and the update they
+// serve is small against the weight.
+__device__ __forceinline__ float rcp_fast(float x) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+// One element, fp32 moments; g: scaled gradient.  The divisor is 0 or at least
+// the smallest normal number (the host checks eps).
+__device__ __forceinline__ void update1(const AdamWArgs &a, float decay, float g, float &w, float &m,
+                                        float &v) {
   m = __fadd_rn(__fmul_rn(m, a.beta1), __fmul_rn(g, a.omb1));
   v = __fadd_rn(__fmul_rn(v, a.beta2), __fmul_rn(__fmul_rn(g, g), a.omb2));
-}
-__device__ __forceinline__ float step_w(const AdamWArgs &a, float decay, float w, float m, float r) {
+  float r;
+  asm("sqrt.approx.f32 %0, %1;" : "=f"(r) : "f"(v));
   const float den = __fadd_rn(__fmul_rn(r, a.rs2), a.eps);
-  return __fsub_rn(__fmul_rn(w, decay), __fdiv_rn(__fmul_rn(m, a.c1), den));
+  w = __fadd_rn(__fmul_rn(w, decay), __fmul_rn(__fmul_rn(m, a.neg_c1), rcp_fast(den)));
 }
 
+// With 8-bit moments the instructions, not the bytes, bound the kernel: two
+// elements per instruction (f32x2), sums of products as multiply-adds.  (The
+// compiler fuses a packed multiply into a packed add whatever their rounding
+// modifiers say, so the fused form is what is written.)
+typedef unsigned long long Pair;
+__device__ __forceinline__ Pair pair(float a, float b) {
+  Pair p;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(p) : "f"(a), "f"(b));
+  return p;
+}
+__device__ __forceinline__ void unpair(Pair p, float &a, float &b) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(p));
+}
+__device__ __forceinline__ Pair mul2(Pair a, Pair b) {
+  Pair p;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(p) : "l"(a), "l"(b));
+  return p;
+}
+__device__ __forceinline__ Pair fma2(Pair a, Pair b, Pair c) {
+  Pair p;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(p) : "l"(a), "l"(b), "l"(c));
+  return p;
+}
+__device__ __forceinline__ Pair twice(float a) { return pair(a, a); }
+__device__ __forceinline__ Pair step_w(const AdamWArgs &a, float decay, Pair w, Pair m, Pair r) {
+  float d0, d1;
+  unpair(fma2(r, twice(a.rs2), twice(a.eps)), d0, d1);
+  return fma2(w, twice(decay), mul2(mul2(m, twice(a.neg_c1)), pair(rcp_fast(d0), rcp_fast(d1))));
+}
+// The root as the state keeps it, rounded to nearest: the hardware's reciprocal
+// root y of v and one Newton step r + (v - r^2) y / 2 from r = v y, whose residual
+// the multiply-add leaves exact.  Small v are scaled by 2^64 to keep it so; 0, inf
+// and nan are their own results.
+__device__ __forceinline__ Pair root_near(Pair v) {
+  float v0, v1;
+  unpair(v, v0, v1);
+  const bool s0 = v0 < 0x1p-64f, s1 = v1 < 0x1p-64f;
+  const float x0 = s0 ? v0 * 0x1p64f : v0, x1 = s1 ? v1 * 0x1p64f : v1;
+  float y0, y1, r0, r1;
+  asm("rsqrt.approx.ftz.f32 %0, %1;" : "=f"(y0) : "f"(x0));
+  asm("rsqrt.approx.ftz.f32 %0, %1;" : "=f"(y1) : "f"(x1));
+  const Pair x = pair(x0, x1), y = pair(y0, y1);
+  const Pair r = mul2(x, y);
+  unpair(r, r0, r1);
+  const Pair left = fma2(pair(-r0, -r1), r, x);
+  unpair(fma2(left, mul2(y, twice(0.5f)), r), r0, r1);
+  r0 = s0 ? r0 * 0x1p-32f : r0, r1 = s1 ? r1 * 0x1p-32f : r1;
+  r0 = __float_as_uint(v0) - 1u < 0x7f7fffffu ? r0 : v0;
+  r1 = __float_as_uint(v1) - 1u < 0x7f7fffffu ? r1 : v1;
+  return pair(r0, r1);
+}
 // ---- 8-bit codes -----------------------------------------------------------------
 // Multiply and xor-shift rounds; the multipliers are binary fractions of the
 // golden ratio and of the roots of 2, 3 and 5.  Any well-mixed function would do.
+constexpr unsigned kPlaceMul = 0x9E3779B1u, kHighMul = 0x3C6EF373u;
 __host__ __device__ __forceinline__ unsigned mix_bits(unsigned x) {
   x = (x ^ (x >> 16)) * 0x6A09E667u;
   x = (x ^ (x >> 15)) * 0xBB67AE85u;
   return x ^ (x >> 16);
 }
-__device__ __forceinline__ unsigned rounding_bits(unsigned long long place, unsigned key) {
-  return mix_bits((unsigned)place * 0x9E3779B1u + (unsigned)(place >> 32) * 0x3C6EF373u + key);
-}
-// A code's 7 magnitude bits lead a float's exponent and mantissa, which is the
-// same number times 2^-120, subnormals included.
-__device__ __forceinline__ float decode(unsigned code, float scale) {
-  const unsigned bits = ((code & 0x7fu) << 20) | ((code & 0x80u) << 24);
-  return __fmul_rn(__fmul_rn(__uint_as_float(bits), 0x1p120f), scale);
+// Two code bytes (the low 16 bits) as numbers.
+__device__ __forceinline__ Pair decode2(unsigned codes) {
+  unsigned h;
+  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"((unsigned short)codes));
+  const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&h));
+  return pair(f.x, f.y);
 }
 __device__ __forceinline__ float scale_of(unsigned byte) {
   return byte == 0 ? 0x1p-127f : __uint_as_float(byte == 255 ? 0x7fc00000u : byte << 23);
 }
-// Scale byte of a block with this largest magnitude (as bits), and the scale's
-// inverse: the block's largest code lies in [128, 256), which leaves room to
-// round up below 448.  255 (not a number) for a block that holds inf or nan.
-__device__ __forceinline__ unsigned block_scale(unsigned max_bits, float &inverse) {
+// A block's scale byte and what to multiply its values by before `encode`, from
+// the largest magnitude (as bits) of the block: the largest code lies in [128, 256),
+// which leaves room to round up below 448.  255 (not a number): the block holds inf
+// or nan.  The factor, 2^(7 - e - 120), is no float for the largest e: `big` says
+// that the values are to be multiplied by 2^-100 first.
+struct BlockScale {
+  unsigned byte;
+  bool big;
+  float factor;
+};
+__device__ __forceinline__ BlockScale block_scale(unsigned max_bits) {
   unsigned e = max_bits >> 23;
   e = e < 8u ? 8u : e > 254u ? 254u : e;
-  inverse = __uint_as_float((261u - e) << 23);
-  return max_bits >= 0x7f800000u ? 255u : e - 7u;
+  BlockScale b;
+  b.byte = max_bits >= 0x7f800000u ? 255u : e - 7u;
+  b.big = e > 140u;
+  b.factor = __uint_as_float((141u - (b.big ? e - 100u : e)) << 23);
+  return b;
 }
-// 20 random bits: 16 of the hash, then a one that centres them, then zeros.
-__device__ __forceinline__ unsigned encode(float x, float inverse, unsigned bits16) {
-  const float y = __fmul_rn(__fmul_rn(fabsf(x), inverse), 0x1p-120f);
-  return ((__float_as_uint(y) + ((bits16 << 4) | 8u)) >> 20) | ((__float_as_uint(x) >> 24) & 0x80u);
+// The code's magnitude in the low 7 bits of x times the block's factor: its bits lead
+// the float's, subnormal ones included; 20 random bits below them are added: 16 of the
+// hash, then a one that centres them, then zeros.
+__device__ __forceinline__ unsigned encode(float scaled, unsigned bits16) {
+  return (__float_as_uint(scaled) + ((bits16 << 4) | 8u)) >> 20;
 }
 
 // ---- one unit: eight elements per lane ---------------------------------------------
@@ -146,54 +222,52 @@ template <int RB, typename GT>
 __device__ __forceinline__ void unit_vec(const View<RB> &t, const AdamWArgs &a, int R, float s,
                                          float decay, size_t i, float *m_, float *v_) {
   const int lane = threadIdx.x & 31;
-  float g[2][4], w[2][4], m[2][4], v[2][4];
+  float g[2][4];
+  float4 w[2], m[2], v[2];
 #pragma unroll
   for (int q = 0; q < 2; ++q) {
     const int o = 4 * lane + 128 * q;
     sum_grad4<RB, GT>(t.g, R, i + o, g[q]);
-    const float4 w4 = *reinterpret_cast<const float4 *>(t.w + i + o);
-    const float4 m4 = *reinterpret_cast<const float4 *>(m_ + o);
-    const float4 v4 = *reinterpret_cast<const float4 *>(v_ + o);
-    w[q][0] = w4.x, w[q][1] = w4.y, w[q][2] = w4.z, w[q][3] = w4.w;
-    m[q][0] = m4.x, m[q][1] = m4.y, m[q][2] = m4.z, m[q][3] = m4.w;
-    v[q][0] = v4.x, v[q][1] = v4.y, v[q][2] = v4.z, v[q][3] = v4.w;
+    w[q] = *reinterpret_cast<const float4 *>(t.w + i + o);
+    m[q] = *reinterpret_cast<const float4 *>(m_ + o);
+    v[q] = *reinterpret_cast<const float4 *>(v_ + o);
   }
 #pragma unroll
   for (int q = 0; q < 2; ++q) {
     const int o = 4 * lane + 128 * q;
+    float w4[4] = {w[q].x, w[q].y, w[q].z, w[q].w}, m4[4] = {m[q].x, m[q].y, m[q].z, m[q].w},
+          v4[4] = {v[q].x, v[q].y, v[q].z, v[q].w};
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      moments(a, __fmul_rn(g[q][e], s), m[q][e], v[q][e]);
-      w[q][e] = step_w(a, decay, w[q][e], m[q][e], __fsqrt_rn(v[q][e]));
-    }
-    *reinterpret_cast<float4 *>(m_ + o) = make_float4(m[q][0], m[q][1], m[q][2], m[q][3]);
-    *reinterpret_cast<float4 *>(v_ + o) = make_float4(v[q][0], v[q][1], v[q][2], v[q][3]);
-    put_w4<RB>(t, R, a.lp_kind, i + o, w[q]);
+    for (int e = 0; e < 4; ++e) update1(a, decay, __fmul_rn(g[q][e], s), w4[e], m4[e], v4[e]);
+    *reinterpret_cast<float4 *>(m_ + o) = make_float4(m4[0], m4[1], m4[2], m4[3]);
+    *reinterpret_cast<float4 *>(v_ + o) = make_float4(v4[0], v4[1], v4[2], v4[3]);
+    put_w4<RB>(t, R, a.lp_kind, i + o, w4);
   }
 }
-// Scalar form: nv elements of this lane, `stride` apart.
-template <int RB, typename GT>
+// Scalar form: nv (0..8) elements of this lane, STRIDE apart, four at a time.
+template <int RB, typename GT, int STRIDE>
 __device__ __forceinline__ void unit_scalar(const View<RB> &t, const AdamWArgs &a, int R, float s,
-                                            float decay, size_t i, int stride, int nv, float *m_,
-                                            float *v_) {
-  float g[8], w[8], m[8], v[8];
+                                            float decay, size_t i, int nv, float *m_, float *v_) {
+#pragma unroll 1
+  for (int q = 0; q < nv; q += 4, i += 4 * STRIDE, m_ += 4 * STRIDE, v_ += 4 * STRIDE) {
+    float g[4], w[4], m[4], v[4];
 #pragma unroll
-  for (int e = 0; e < 8; ++e)
-    if (e < nv) {
-      g[e] = sum_grad1<RB, GT>(t.g, R, i + e * stride);
-      w[e] = t.w[i + e * stride];
-      m[e] = m_[e * stride];
-      v[e] = v_[e * stride];
-    }
+    for (int e = 0; e < 4; ++e)
+      if (q + e < nv) {
+        g[e] = sum_grad1<RB, GT>(t.g, R, i + e * STRIDE);
+        w[e] = t.w[i + e * STRIDE];
+        m[e] = m_[e * STRIDE];
+        v[e] = v_[e * STRIDE];
+      }
 #pragma unroll
-  for (int e = 0; e < 8; ++e)
-    if (e < nv) {
-      moments(a, __fmul_rn(g[e], s), m[e], v[e]);
-      w[e] = step_w(a, decay, w[e], m[e], __fsqrt_rn(v[e]));
-      m_[e * stride] = m[e];
-      v_[e * stride] = v[e];
-      put_w1<RB>(t, R, a.lp_kind, i + e * stride, w[e]);
-    }
+    for (int e = 0; e < 4; ++e)
+      if (q + e < nv) {
+        update1(a, decay, __fmul_rn(g[e], s), w[e], m[e], v[e]);
+        m_[e * STRIDE] = m[e];
+        v_[e * STRIDE] = v[e];
+        put_w1<RB>(t, R, a.lp_kind, i + e * STRIDE, w[e]);
+      }
+  }
 }
 
 // 8-bit state.  VEC: elements as in unit_vec, codes read and written four at a
@@ -205,8 +279,9 @@ __device__ __forceinline__ void unit_quant(const View<RB> &t, const AdamWArgs &a
                                            unsigned char *scale) {
   const int lane = threadIdx.x & 31;
   auto at = [&](int e) { return VEC ? 4 * lane + (e & 3) + 128 * (e >> 2) : lane + 32 * e; };
+  auto have = [&](int e) { return VEC || at(e) < avail; };
   float g[8], w[8], m[8], r[8];
-  unsigned mc[2], rc[2];  // VEC: four codes each
+  unsigned mc[4], rc[4];  // two codes each
   const unsigned sc = *reinterpret_cast<const unsigned short *>(scale);
   if constexpr (VEC) {
 #pragma unroll
@@ -215,39 +290,43 @@ __device__ __forceinline__ void unit_quant(const View<RB> &t, const AdamWArgs &a
       float g4[4];
       sum_grad4<RB, GT>(t.g, R, i + o, g4);
       const float4 w4 = *reinterpret_cast<const float4 *>(t.w + i + o);
-      mc[q] = *reinterpret_cast<const unsigned *>(m_ + o);
-      rc[q] = *reinterpret_cast<const unsigned *>(r_ + o);
+      const unsigned m4 = *reinterpret_cast<const unsigned *>(m_ + o);
+      const unsigned r4 = *reinterpret_cast<const unsigned *>(r_ + o);
+      mc[2 * q] = m4 & 0xffffu, mc[2 * q + 1] = m4 >> 16;
+      rc[2 * q] = r4 & 0xffffu, rc[2 * q + 1] = r4 >> 16;
 #pragma unroll
       for (int e = 0; e < 4; ++e) g[4 * q + e] = g4[e];
       w[4 * q] = w4.x, w[4 * q + 1] = w4.y, w[4 * q + 2] = w4.z, w[4 * q + 3] = w4.w;
     }
   } else {
 #pragma unroll
-    for (int e = 0; e < 8; ++e)
-      if (at(e) < avail) {
-        g[e] = sum_grad1<RB, GT>(t.g, R, i + at(e));
-        w[e] = t.w[i + at(e)];
-        m[e] = __uint_as_float(m_[at(e)]);
-        r[e] = __uint_as_float(r_[at(e)]);
-      }
+    for (int e = 0; e < 8; ++e) {
+      g[e] = have(e) ? sum_grad1<RB, GT>(t.g, R, i + at(e)) : 0.f;
+      w[e] = have(e) ? t.w[i + at(e)] : 0.f;
+      const unsigned cm = have(e) ? m_[at(e)] : 0u, cr = have(e) ? r_[at(e)] : 0u;
+      mc[e >> 1] = e & 1 ? mc[e >> 1] | (cm << 8) : cm;
+      rc[e >> 1] = e & 1 ? rc[e >> 1] | (cr << 8) : cr;
+    }
   }
   const float m_scale = scale_of(sc & 0xffu), r_scale = scale_of(sc >> 8);
   unsigned m_max = 0, r_max = 0;
 #pragma unroll
-  for (int e = 0; e < 8; ++e)
-    if (VEC || at(e) < avail) {
-      const unsigned cm = VEC ? (mc[e >> 2] >> (8 * (e & 3))) & 0xffu : __float_as_uint(m[e]);
-      const unsigned cr = VEC ? (rc[e >> 2] >> (8 * (e & 3))) & 0xffu : __float_as_uint(r[e]);
-      m[e] = decode(cm, m_scale);
-      const float r0 = decode(cr, r_scale);
-      float v = __fmul_rn(r0, r0);
-      moments(a, __fmul_rn(g[e], s), m[e], v);
-      r[e] = __fsqrt_rn(v);
-      w[e] = step_w(a, decay, w[e], m[e], r[e]);
-      const unsigned mb = __float_as_uint(m[e]) & 0x7fffffffu, rb = __float_as_uint(r[e]) & 0x7fffffffu;
-      m_max = mb > m_max ? mb : m_max;
-      r_max = rb > r_max ? rb : r_max;
-    }
+  for (int e = 0; e < 8; e += 2) {
+    Pair pm = mul2(decode2(mc[e >> 1]), twice(m_scale));
+    const Pair r0 = mul2(decode2(rc[e >> 1]), twice(r_scale));
+    const Pair pg = mul2(pair(g[e], g[e + 1]), twice(s));
+    pm = fma2(pm, twice(a.beta1), mul2(pg, twice(a.omb1)));
+    const Pair pr = root_near(fma2(mul2(r0, r0), twice(a.beta2), mul2(mul2(pg, pg), twice(a.omb2))));
+    unpair(step_w(a, decay, pair(w[e], w[e + 1]), pm, pr), w[e], w[e + 1]);
+    unpair(pm, m[e], m[e + 1]);
+    unpair(pr, r[e], r[e + 1]);
+#pragma unroll
+    for (int k = e; k < e + 2; ++k)
+      if (have(k)) {
+        m_max = max(m_max, __float_as_uint(m[k]) & 0x7fffffffu);
+        r_max = max(r_max, __float_as_uint(r[k]) & 0x7fffffffu);
+      }
+  }
   if constexpr (VEC) {
 #pragma unroll
     for (int q = 0; q < 2; ++q) {
@@ -257,23 +336,41 @@ __device__ __forceinline__ void unit_quant(const View<RB> &t, const AdamWArgs &a
   } else {
 #pragma unroll
     for (int e = 0; e < 8; ++e)
-      if (at(e) < avail) put_w1<RB>(t, R, a.lp_kind, i + at(e), w[e]);
+      if (have(e)) put_w1<RB>(t, R, a.lp_kind, i + at(e), w[e]);
   }
-  m_max = __reduce_max_sync(0xffffffffu, m_max);
-  r_max = __reduce_max_sync(0xffffffffu, r_max);
-  float m_inv, r_inv;
-  const unsigned mb = block_scale(m_max, m_inv), rb = block_scale(r_max, r_inv);
+  const BlockScale mb = block_scale(__reduce_max_sync(0xffffffffu, m_max));
+  const BlockScale rb = block_scale(__reduce_max_sync(0xffffffffu, r_max));
+  if (mb.big) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) m[e] *= 0x1p-100f;
+  }
+  if (rb.big) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) r[e] = r[e] > 0.f ? fmaxf(r[e] * 0x1p-100f, 0x1p-126f) : r[e];  // stays positive
+  }
+  // place * multiplier + key, stepped from element to element
+  const unsigned first = (unsigned)(place + at(0)) * kPlaceMul + (unsigned)((place + at(0)) >> 32) * kHighMul + a.key;
   unsigned cm[8], cr[8];
 #pragma unroll
-  for (int e = 0; e < 8; ++e)
-    if (VEC || at(e) < avail) {
-      const unsigned bits = rounding_bits(place + at(e), a.key);
-      const unsigned x = encode(m[e], m_inv, bits & 0xffffu);
-      unsigned y = encode(r[e], r_inv, bits >> 16);
-      if (y == 0u && r[e] > 0.f) y = 1u;
-      cm[e] = mb == 255u ? 0u : x;
-      cr[e] = rb == 255u ? 0u : y;
+  for (int e = 0; e < 8; e += 2) {
+    float y[2], z[2];
+    unpair(mul2(pair(fabsf(m[e]), fabsf(m[e + 1])), twice(mb.factor)), y[0], y[1]);
+    unpair(mul2(pair(r[e], r[e + 1]), twice(rb.factor)), z[0], z[1]);
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      const unsigned bits = mix_bits(first + (unsigned)(at(e + k) - at(0)) * kPlaceMul);
+      cm[e + k] = encode(y[k], bits & 0xffffu) | ((__float_as_uint(m[e + k]) >> 24) & 0x80u);
+      const unsigned c = encode(z[k], bits >> 16);
+      cr[e + k] = r[e + k] > 0.f ? max(c, 1u) : c;
     }
+  }
+  if (mb.byte == 255u || rb.byte == 255u) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      if (mb.byte == 255u) cm[e] = 0u;
+      if (rb.byte == 255u) cr[e] = 0u;
+    }
+  }
   if constexpr (VEC) {
 #pragma unroll
     for (int q = 0; q < 2; ++q) {
@@ -286,9 +383,9 @@ __device__ __forceinline__ void unit_quant(const View<RB> &t, const AdamWArgs &a
   } else {
 #pragma unroll
     for (int e = 0; e < 8; ++e)
-      if (at(e) < avail) m_[at(e)] = (unsigned char)cm[e], r_[at(e)] = (unsigned char)cr[e];
+      if (have(e)) m_[at(e)] = (unsigned char)cm[e], r_[at(e)] = (unsigned char)cr[e];
   }
-  if (lane == 0) *reinterpret_cast<unsigned short *>(scale) = (unsigned short)(mb | (rb << 8));
+  if (lane == 0) *reinterpret_cast<unsigned short *>(scale) = (unsigned short)(mb.byte | (rb.byte << 8));
 }
 
 // A unit inside one tensor: `avail` (1..256) elements from element i of the
@@ -310,8 +407,8 @@ __device__ __forceinline__ void unit_inside(const View<RB> &t, const AdamWArgs &
     if (vec && avail == kListUnit)
       unit_vec<RB, GT>(t, a, R, s, decay, i, m, v);
     else
-      unit_scalar<RB, GT>(t, a, R, s, decay, i + lane, 32, avail > lane ? (avail - lane + 31) / 32 : 0,
-                          m + lane, v + lane);
+      unit_scalar<RB, GT, 32>(t, a, R, s, decay, i + lane, avail > lane ? (avail - lane + 31) / 32 : 0,
+                              m + lane, v + lane);
   }
 }
 
@@ -364,9 +461,9 @@ __global__ void __launch_bounds__(COCO_ADAMW_THREADS, 2)
         View<1> tl;
         tl.g[0] = tab.g[k], tl.w = tab.w[k], tl.lp = tab.lp[k];
         const int nv = el + 1 < s_off[k + 1] ? kListGroup : kListGroup - tab.missing[k];
-        unit_scalar<1, GT>(tl, a, 1, s, tab.decays[k] ? a.decay : 1.f,
-                           (size_t)(el - s_off[k]) * kListGroup, 1, nv,
-                           (float *)a.m + (size_t)el * kListGroup, (float *)a.v + (size_t)el * kListGroup);
+        unit_scalar<1, GT, 1>(tl, a, 1, s, tab.decays[k] ? a.decay : 1.f,
+                              (size_t)(el - s_off[k]) * kListGroup, nv,
+                              (float *)a.m + (size_t)el * kListGroup, (float *)a.v + (size_t)el * kListGroup);
       }
       __syncwarp();
     }
@@ -408,10 +505,10 @@ __global__ void __launch_bounds__(COCO_ADAMW_PEER_THREADS, 2)
         const PeerPiece &pl = pieces[bisect(k, n - 1, el, [&](int x) { return pieces[x].off; })];
         const size_t done = (size_t)(el - pl.off) * kListGroup, left = (size_t)pl.len - done;
         const View<RB> t = {pl.g, pl.out, pl.w};
-        unit_scalar<RB, GT>(t, a, R, s, pl.decays ? a.decay : 1.f, (size_t)pl.begin + done, 1,
-                            left < kListGroup ? (int)left : kListGroup,
-                            (float *)a.m + (size_t)el * kListGroup,
-                            (float *)a.v + (size_t)el * kListGroup);
+        unit_scalar<RB, GT, 1>(t, a, R, s, pl.decays ? a.decay : 1.f, (size_t)pl.begin + done,
+                               left < kListGroup ? (int)left : kListGroup,
+                               (float *)a.m + (size_t)el * kListGroup,
+                               (float *)a.v + (size_t)el * kListGroup);
       }
       __syncwarp();
     }
@@ -448,8 +545,8 @@ PeerKernel pick_peer(bool quant, cocoDataType_t g, int world) {
 }  // namespace
 
 unsigned adamw_rounding_key(uint64_t seed, int step) {
-  return mix_bits(mix_bits((unsigned)seed) + (unsigned)(seed >> 32) * 0x3C6EF373u +
-                  (unsigned)step * 0x9E3779B1u);
+  return mix_bits(mix_bits((unsigned)seed) + (unsigned)(seed >> 32) * kHighMul +
+                  (unsigned)step * kPlaceMul);
 }
 
 int adamw_threads(bool, cocoDataType_t) { return COCO_ADAMW_THREADS; }

@@ -47,7 +47,7 @@ struct AdamWArgs {
   int state_aligned;             // m and v (codes) allow the vector path
   unsigned key;                  // of the rounding bits
   float grad_scale, beta1, beta2, omb1, omb2;
-  float c1;                      // lr / (1 - beta1^t)
+  float neg_c1;                  // -lr / (1 - beta1^t)
   float rs2;                     // 1 / sqrt(1 - beta2^t)
   float eps, decay;              // decay: 1 - lr * weight_decay
 };

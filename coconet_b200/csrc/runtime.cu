@@ -17,6 +17,7 @@
 #include <unistd.h>
 
 #include <algorithm>
+#include <cfloat>
 #include <cmath>
 #include <map>
 #include <memory>
@@ -1960,6 +1961,7 @@ static int adamw_call(ListCall *lc, cocoComm_t comm, size_t nbuff, const void *c
                       cocoStream_t stream) {
   if (!comm || nbuff == 0 || !g || !w || !counts || step < 0) return cocoInvalidArgument;
   if (!(beta1 >= 0.f && beta1 < 1.f && beta2 >= 0.f && beta2 < 1.f && eps >= 0.f)) return cocoInvalidArgument;
+  if (eps != 0.f && eps < FLT_MIN) return cocoInvalidArgument;  // the kernels divide by it as a normal number
   if (!std::isfinite(lr) || !std::isfinite(weight_decay) || !std::isfinite(eps) || !std::isfinite(grad_scale))
     return cocoInvalidArgument;
   lc->n = nbuff, lc->g = g, lc->g_type = g_type, lc->w = w, lc->lp = w_lp, lc->lp_type = lp_type;
@@ -1970,7 +1972,7 @@ static int adamw_call(ListCall *lc, cocoComm_t comm, size_t nbuff, const void *c
   const double d1 = 1.0 - std::pow((double)beta1, t), d2 = 1.0 - std::pow((double)beta2, t);
   a.grad_scale = grad_scale, a.beta1 = beta1, a.beta2 = beta2;
   a.omb1 = 1.0f - beta1, a.omb2 = 1.0f - beta2;
-  a.c1 = (float)((double)lr / d1);
+  a.neg_c1 = (float)(-(double)lr / d1);
   a.rs2 = (float)(1.0 / std::sqrt(d2));
   a.eps = eps;
   a.decay = (float)(1.0 - (double)lr * (double)weight_decay);

@@ -354,14 +354,16 @@ int cocoFusedLAMBScattered(cocoComm_t comm, size_t nbuff, const void *const *g,
  *     g <- (sum over ranks of g) * (norm ? norm[1] * grad_scale : grad_scale)
  *     m <- beta1 m + (1 - beta1) g        v <- beta2 v + (1 - beta2) g^2
  *     w <- w (1 - lr weight_decay) - (lr / d1) m / (sqrt(v) / sqrt(d2) + eps)
- * every operation rounded to fp32.  With `norm` (as cocoGradNormScattered left it
+ * every operation rounded to fp32 (m and v so to the last bit); the root and the
+ * reciprocal in w's update are the hardware's, within 2^-23 each.  With `norm` (as cocoGradNormScattered left it
  * on every rank) whose norm[0] is inf or nan the step changes nothing.
  *   w_lp      NULL, or per tensor a 16-bit copy of w (lp_type), gathered instead
  *             of w; then, as in the flat call, only the own slice of w is updated
  *   no_decay  NULL, or per tensor a byte (host): not 0 = weight_decay does not apply
  *   m, v      as in cocoFusedAdamScattered (cocoScatteredSliceElems elements), and
  *             interchangeable with its moments
- * 0 <= beta < 1, eps >= 0, step >= 0, all finite, else cocoInvalidArgument.
+ * 0 <= beta < 1, eps 0 or a normal fp32 number, step >= 0, all finite, else
+ * cocoInvalidArgument.
  *
  * cocoFusedAdamWQuantScattered: the same step with the moments in 8 bits: m and
  * vroot = sqrt(v) as e4m3 codes (one byte per element), and per COCO_QUANT_BLOCK
@@ -375,7 +377,8 @@ int cocoFusedLAMBScattered(cocoComm_t comm, size_t nbuff, const void *const *g,
  * the probability of the part cut off (to nearest, a beta2 of 0.999 would never
  * move vroot); the random bits are a function of `seed`, `step` and the element's
  * place in the flat state, so that a step is reproducible, and the same at every
- * world size.  A vroot above 0 is never stored as 0; a block in which a moment is
+ * world size.  (m and v are formed with one multiply-add each, not rounded between
+ * the product and the sum.)  A vroot above 0 is never stored as 0; a block in which a moment is
  * inf or nan gets scale byte 255, which reads back as nan. */
 int cocoGradNormScattered(cocoComm_t comm, size_t nbuff, const void *const *g,
                           cocoDataType_t g_type, const size_t *counts, float grad_scale,

@@ -1,6 +1,8 @@
 """Plain evaluations of AdamW and its 8-bit state for the tests: in fp64 from the
 definition, and in fp32 with every operation rounded by itself, which the
-kernels have to match bit for bit.  numpy only."""
+kernels' moments, codes and scales have to match bit for bit.  The weights, whose
+update goes through the hardware's reciprocal and root, have to match it within
+`near32`.  numpy only."""
 import math
 
 import numpy as np
@@ -44,8 +46,8 @@ def bounds64(w, m, v, g, step, decays=True):
       g'  = g s                                   1 rounding
       m'  = (m b1) + (g' omb1)                    u (2 |m b1| + 3 |g omb1|)
       v'  = (v b2) + ((g' g') omb2)               at most 5 roundings of its larger part, no cancellation
-      r   = sqrt(v'), den = r rs2 + eps           2.5 + 1, + 1 (rs2) + 1 + 1: 6.5 u relative
-      q   = (m' c1) / den                         m' error / m' + 3 u + 6.5 u
+      r   = sqrt(v'), den = r rs2 + eps           2.5 + 2 (the hardware's root: 2^-23), + 1 (rs2) + 1 + 1: 7.5 u
+      q   = (m' c1) * (1 / den)                   m' error / m' + 1 (c1) + 1 + 2 (its reciprocal) + 1 + 7.5 u
       w'  = w decay - q                           2 u |w| + error of q + u |w'|
     and 2^-140 for what the smallest numbers lose below the normal range (six places of at most 2^-149)."""
     b1, b2 = float(HYPER["beta1"]), float(HYPER["beta2"])
@@ -57,7 +59,7 @@ def bounds64(w, m, v, g, step, decays=True):
         per_m = np.where(m1 != 0, np.abs(q / np.where(m1 != 0, m1, 1)), 0.0)  # dq / dm
     per_m = np.where(m1 != 0, per_m, float(HYPER["lr"]) / (1 - b1 ** (step + 1)) /
                      (np.sqrt(v1 / (1 - b2 ** (step + 1))) + float(HYPER["eps"])))
-    eq = em * per_m + 1.01 * U * 9.5 * np.abs(q) + tiny
+    eq = em * per_m + 1.01 * U * 12.5 * np.abs(q) + tiny
     ew = 1.01 * U * (2 * np.abs(w) + np.abs(w1)) + eq + tiny
     return ew, em, ev
 
@@ -74,6 +76,23 @@ def moments32(h, m, v, g):
     return m * h["b1"] + g * h["omb1"], v * h["b2"] + (g * g) * h["omb2"]
 
 
+def fma32(a, b, c):
+    """a * b + c rounded once.  The product of two fp32 numbers is exact in fp64; the fp64 sum is rounded to odd
+    (its last bit set when anything was cut off), which makes the second rounding, to fp32, the only one that counts."""
+    p, c = a.astype(np.float64) * float(b), c.astype(np.float64)
+    s = p + c
+    t = s - p
+    cut = (p - (s - t)) + (c - t)
+    even = (s.view(np.uint64) & np.uint64(1)) == 0
+    fix = np.isfinite(s) & (cut != 0) & even
+    return np.where(fix, np.nextafter(s, np.where(cut > 0, np.inf, -np.inf)), s).astype(F)
+
+
+def fused_moments32(h, m, v, g):
+    """The 8-bit form's: the first product goes unrounded into the sum."""
+    return fma32(m, h["b1"], g * h["omb1"]), fma32(v, h["b2"], (g * g) * h["omb2"])
+
+
 def weights32(h, w, m, r, decays):
     return w * (h["decay"] if decays else F(1)) - (m * h["c1"]) / (r * h["rs2"] + h["eps"])
 
@@ -88,6 +107,18 @@ def sum32(grads):
     for g in grads[1:]:
         x = x + g.astype(F)
     return x
+
+
+def near32(got, w, m, v, g, step, decays=True, hyper=HYPER):
+    """Whether the weights `got` are step32's up to the two approximations: w - q with q off by
+    2 u (root) + 2 u (reciprocal) and, as the operations before and after round differently, 4 u more; and the
+    last subtraction half a step of either side.  (m, v, w, g: before the step.)"""
+    w1, m1, v1 = step32(w, m, v, g, step, decays, hyper)
+    with np.errstate(all="ignore"):
+        h = scalars32(step, **hyper)
+        q = np.abs((m1 * h["c1"]) / (np.sqrt(v1) * h["rs2"] + h["eps"])).astype(np.float64)
+        far = np.abs(got.astype(np.float64) - w1.astype(np.float64))
+        return bool((far <= 8 * U * q + 2 * U * np.abs(w1.astype(np.float64)) + 2.0 ** -140).all())
 
 
 def step32(w, m, v, g, step, decays=True, hyper=HYPER):
@@ -157,7 +188,7 @@ def quant_step32(w, m_codes, r_codes, scales, g, step, seed, place, decays=True,
         sc = scale_values(scales).astype(F).repeat(BLOCK, 0)[:w.size]
         m = code_values(m_codes).astype(F) * sc[:, 0]
         r = code_values(r_codes).astype(F) * sc[:, 1]
-        m, v = moments32(h, m, r * r, g)
+        m, v = fused_moments32(h, m, r * r, g)
         r = np.sqrt(v)
         w = weights32(h, w, m, r, decays)
         bits = rounding_bits(place, w.size, seed, step)
