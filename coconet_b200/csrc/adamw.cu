@@ -21,8 +21,31 @@
 // What bounds it: HBM.  One pass, every byte moved once; nothing is reused.
 #include "list_device.cuh"
 
-#ifndef COCO_ADAMW_THREADS
-#define COCO_ADAMW_THREADS 384
+#include <atomic>
+
+#ifndef COCO_ADAMW_THREADS16
+#define COCO_ADAMW_THREADS16 352
+#endif
+#ifndef COCO_ADAMW_CTAS16
+#define COCO_ADAMW_CTAS16 2
+#endif
+#ifndef COCO_ADAMW_THREADS32
+#define COCO_ADAMW_THREADS32 352
+#endif
+#ifndef COCO_ADAMW_CTAS32
+#define COCO_ADAMW_CTAS32 2
+#endif
+#ifndef COCO_ADAMW_PACKED_THREADS
+#define COCO_ADAMW_PACKED_THREADS 512
+#endif
+#ifndef COCO_ADAMW_PACKED_CTAS
+#define COCO_ADAMW_PACKED_CTAS 2
+#endif
+#ifndef COCO_ADAMW_QUANT_THREADS
+#define COCO_ADAMW_QUANT_THREADS 512
+#endif
+#ifndef COCO_ADAMW_QUANT_CTAS
+#define COCO_ADAMW_QUANT_CTAS 2
 #endif
 #ifndef COCO_ADAMW_PEER_THREADS
 #define COCO_ADAMW_PEER_THREADS 256
@@ -43,7 +66,7 @@ template <> struct View<1> {
   void *lp;
 };
 
-template <int RB> __device__ __forceinline__ void put_lp4(const View<RB> &v, int R, int kind, size_t i,
+template <int RB, typename Index> __device__ __forceinline__ void put_lp4(const View<RB> &v, int R, int kind, Index i,
                                                           const float (&x)[4]) {
   uint2 q;
   if (kind == kLpF16) {
@@ -61,7 +84,7 @@ template <int RB> __device__ __forceinline__ void put_lp4(const View<RB> &v, int
       if (RB == 2 || p < R) st_sys_8((unsigned short *)v.out[p] + i, q);
   }
 }
-template <int RB> __device__ __forceinline__ void put_lp1(const View<RB> &v, int R, int kind, size_t i,
+template <int RB, typename Index> __device__ __forceinline__ void put_lp1(const View<RB> &v, int R, int kind, Index i,
                                                           float x) {
   const unsigned short h =
       kind == kLpF16 ? Bits16<__half>::from_f32(x) : Bits16<__nv_bfloat16>::from_f32(x);
@@ -73,7 +96,7 @@ template <int RB> __device__ __forceinline__ void put_lp1(const View<RB> &v, int
 }
 // New weights: the own fp32 values and the copy for everybody, or, without a
 // copy, the fp32 values for everybody.
-template <int RB> __device__ __forceinline__ void put_w4(const View<RB> &v, int R, int kind, size_t i,
+template <int RB, typename Index> __device__ __forceinline__ void put_w4(const View<RB> &v, int R, int kind, Index i,
                                                          const float (&x)[4]) {
   if (RB == 1 || kind != kLpNone)
     *reinterpret_cast<float4 *>(v.w + i) = make_float4(x[0], x[1], x[2], x[3]);
@@ -87,7 +110,7 @@ template <int RB> __device__ __forceinline__ void put_w4(const View<RB> &v, int 
       if (RB == 2 || p < R) st_sys_16((float *)v.out[p] + i, q);
   }
 }
-template <int RB> __device__ __forceinline__ void put_w1(const View<RB> &v, int R, int kind, size_t i,
+template <int RB, typename Index> __device__ __forceinline__ void put_w1(const View<RB> &v, int R, int kind, Index i,
                                                          float x) {
   if (RB == 1 || kind != kLpNone) v.w[i] = x;
   if (kind != kLpNone) {
@@ -143,33 +166,27 @@ __device__ __forceinline__ Pair fma2(Pair a, Pair b, Pair c) {
   return p;
 }
 __device__ __forceinline__ Pair twice(float a) { return pair(a, a); }
-__device__ __forceinline__ Pair step_w(const AdamWArgs &a, float decay, Pair w, Pair m, Pair r) {
-  float d0, d1;
-  unpair(fma2(r, twice(a.rs2), twice(a.eps)), d0, d1);
-  return fma2(w, twice(decay), mul2(mul2(m, twice(a.neg_c1)), pair(rcp_fast(d0), rcp_fast(d1))));
+// Of -v, the negative of the root as the state keeps it, rounded to nearest: with y
+// the hardware's reciprocal root of v, one Newton step r + (v - r^2) y / 2 from
+// r = v y.  The multiply-add leaves the residual exact for v from 2^-100 on; 0 gives 0.
+// (Negative throughout, so that no operand has to be negated.)
+__device__ __forceinline__ Pair neg_root(Pair neg_v) {
+  float v0, v1, y0, y1;
+  unpair(neg_v, v0, v1);
+  asm("rsqrt.approx.ftz.f32 %0, %1;" : "=f"(y0) : "f"(fmaxf(-v0, 0x1p-100f)));
+  asm("rsqrt.approx.ftz.f32 %0, %1;" : "=f"(y1) : "f"(fmaxf(-v1, 0x1p-100f)));
+  const Pair y = pair(y0, y1), r = mul2(neg_v, y);
+  return fma2(fma2(r, r, neg_v), mul2(y, twice(0.5f)), r);
 }
-// The root as the state keeps it, rounded to nearest: the hardware's reciprocal
-// root y of v and one Newton step r + (v - r^2) y / 2 from r = v y, whose residual
-// the multiply-add leaves exact.  Small v are scaled by 2^64 to keep it so; 0, inf
-// and nan are their own results.
-__device__ __forceinline__ Pair root_near(Pair v) {
-  float v0, v1;
-  unpair(v, v0, v1);
-  const bool s0 = v0 < 0x1p-64f, s1 = v1 < 0x1p-64f;
-  const float x0 = s0 ? v0 * 0x1p64f : v0, x1 = s1 ? v1 * 0x1p64f : v1;
-  float y0, y1, r0, r1;
-  asm("rsqrt.approx.ftz.f32 %0, %1;" : "=f"(y0) : "f"(x0));
-  asm("rsqrt.approx.ftz.f32 %0, %1;" : "=f"(y1) : "f"(x1));
-  const Pair x = pair(x0, x1), y = pair(y0, y1);
-  const Pair r = mul2(x, y);
-  unpair(r, r0, r1);
-  const Pair left = fma2(pair(-r0, -r1), r, x);
-  unpair(fma2(left, mul2(y, twice(0.5f)), r), r0, r1);
-  r0 = s0 ? r0 * 0x1p-32f : r0, r1 = s1 ? r1 * 0x1p-32f : r1;
-  r0 = __float_as_uint(v0) - 1u < 0x7f7fffffu ? r0 : v0;
-  r1 = __float_as_uint(v1) - 1u < 0x7f7fffffu ? r1 : v1;
-  return pair(r0, r1);
+// The same for any v: small ones scaled up first; inf and nan are their own roots.
+__device__ __forceinline__ float neg_root_any(float neg_v) {
+  const bool small = -neg_v < 0x1p-64f;
+  float r, other;
+  unpair(neg_root(pair(small ? neg_v * 0x1p64f : neg_v, 0.f)), r, other);
+  if (small) r *= 0x1p-32f;
+  return -neg_v < __uint_as_float(0x7f800000u) ? r : neg_v;
 }
+
 // ---- 8-bit codes -----------------------------------------------------------------
 // Multiply and xor-shift rounds; the multipliers are binary fractions of the
 // golden ratio and of the roots of 2, 3 and 5.  Any well-mixed function would do.
@@ -189,11 +206,11 @@ __device__ __forceinline__ Pair decode2(unsigned codes) {
 __device__ __forceinline__ float scale_of(unsigned byte) {
   return byte == 0 ? 0x1p-127f : __uint_as_float(byte == 255 ? 0x7fc00000u : byte << 23);
 }
-// A block's scale byte and what to multiply its values by before `encode`, from
-// the largest magnitude (as bits) of the block: the largest code lies in [128, 256),
-// which leaves room to round up below 448.  255 (not a number): the block holds inf
-// or nan.  The factor, 2^(7 - e - 120), is no float for the largest e: `big` says
-// that the values are to be multiplied by 2^-100 first.
+// A block's scale byte and what to multiply its values by before they are rounded,
+// from the largest magnitude (as bits) of the block: the largest code lies in
+// [128, 256), which leaves room to round up below 448.  255 (not a number): the block
+// holds inf or nan.  The factor, 2^(7 - e - 120), is no float for the largest e: `big`
+// says that the values are to be multiplied by 2^-100 first.
 struct BlockScale {
   unsigned byte;
   bool big;
@@ -208,184 +225,247 @@ __device__ __forceinline__ BlockScale block_scale(unsigned max_bits) {
   b.factor = __uint_as_float((141u - (b.big ? e - 100u : e)) << 23);
   return b;
 }
-// The code's magnitude in the low 7 bits of x times the block's factor: its bits lead
-// the float's, subnormal ones included; 20 random bits below them are added: 16 of the
-// hash, then a one that centres them, then zeros.
-__device__ __forceinline__ unsigned encode(float scaled, unsigned bits16) {
-  return (__float_as_uint(scaled) + ((bits16 << 4) | 8u)) >> 20;
+// x times the block's factor has the code's 7 magnitude bits on top of 20 others,
+// subnormal codes included; adding 20 random bits (16 of the hash, a one that centres
+// them, zeros) and cutting 20 off rounds up with the probability of the part cut off.
+// These put the code in the top byte; the sign stays in place.
+__device__ __forceinline__ unsigned code_m(float scaled, unsigned hash) {
+  const unsigned u = __float_as_uint(scaled) + (((hash << 4) & 0xffff0u) | 8u);
+  return (u & 0x80000000u) | ((u << 4) & 0x7fffffffu);
+}
+__device__ __forceinline__ unsigned code_r(float scaled, unsigned hash) {
+  return (__float_as_uint(scaled) + (((hash >> 12) & 0xffff0u) | 8u)) << 4;
+}
+__device__ __forceinline__ unsigned top_bytes(unsigned a, unsigned b, unsigned c, unsigned d) {
+  return __byte_perm(__byte_perm(a, b, 0x0073), __byte_perm(c, d, 0x0073), 0x5410);
+}
+// Largest magnitude of three, nan if one is.
+__device__ __forceinline__ float max_abs(float a, float b, float c) {
+  float d;
+  asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
 }
 
 // ---- one unit: eight elements per lane ---------------------------------------------
 // Vector form: elements i + 4 lane .. + 3 and i + 128 + 4 lane .. + 3, so that
 // every 16-byte access of the warp is one run of memory.
-template <int RB, typename GT>
+// im: of the state.
+template <int RB, typename GT, typename Index>
 __device__ __forceinline__ void unit_vec(const View<RB> &t, const AdamWArgs &a, int R, float s,
-                                         float decay, size_t i, float *m_, float *v_) {
-  const int lane = threadIdx.x & 31;
+                                         float decay, Index i, float *m_, float *v_, Index im) {
+  const unsigned lane = threadIdx.x & 31;
   float g[2][4];
   float4 w[2], m[2], v[2];
 #pragma unroll
   for (int q = 0; q < 2; ++q) {
-    const int o = 4 * lane + 128 * q;
+    const Index o = 4 * lane + 128 * q;
     sum_grad4<RB, GT>(t.g, R, i + o, g[q]);
-    w[q] = *reinterpret_cast<const float4 *>(t.w + i + o);
-    m[q] = *reinterpret_cast<const float4 *>(m_ + o);
-    v[q] = *reinterpret_cast<const float4 *>(v_ + o);
+    w[q] = *reinterpret_cast<const float4 *>(t.w + (i + o));
+    m[q] = *reinterpret_cast<const float4 *>(m_ + (im + o));
+    v[q] = *reinterpret_cast<const float4 *>(v_ + (im + o));
   }
 #pragma unroll
   for (int q = 0; q < 2; ++q) {
-    const int o = 4 * lane + 128 * q;
+    const Index o = 4 * lane + 128 * q;
     float w4[4] = {w[q].x, w[q].y, w[q].z, w[q].w}, m4[4] = {m[q].x, m[q].y, m[q].z, m[q].w},
           v4[4] = {v[q].x, v[q].y, v[q].z, v[q].w};
 #pragma unroll
     for (int e = 0; e < 4; ++e) update1(a, decay, __fmul_rn(g[q][e], s), w4[e], m4[e], v4[e]);
-    *reinterpret_cast<float4 *>(m_ + o) = make_float4(m4[0], m4[1], m4[2], m4[3]);
-    *reinterpret_cast<float4 *>(v_ + o) = make_float4(v4[0], v4[1], v4[2], v4[3]);
+    *reinterpret_cast<float4 *>(m_ + (im + o)) = make_float4(m4[0], m4[1], m4[2], m4[3]);
+    *reinterpret_cast<float4 *>(v_ + (im + o)) = make_float4(v4[0], v4[1], v4[2], v4[3]);
     put_w4<RB>(t, R, a.lp_kind, i + o, w4);
   }
 }
-// Scalar form: nv (0..8) elements of this lane, STRIDE apart, four at a time.
-template <int RB, typename GT, int STRIDE>
+// Scalar form: nv (0..8) elements of this lane, STRIDE apart, four at a time; ALL: eight.
+template <int RB, typename GT, int STRIDE, bool ALL, typename Index>
 __device__ __forceinline__ void unit_scalar(const View<RB> &t, const AdamWArgs &a, int R, float s,
-                                            float decay, size_t i, int nv, float *m_, float *v_) {
+                                            float decay, Index i, int nv, float *m_, float *v_, Index im) {
 #pragma unroll 1
-  for (int q = 0; q < nv; q += 4, i += 4 * STRIDE, m_ += 4 * STRIDE, v_ += 4 * STRIDE) {
+  for (int q = 0; q < (ALL ? 8 : nv); q += 4, i += 4 * STRIDE, im += 4 * STRIDE) {
     float g[4], w[4], m[4], v[4];
 #pragma unroll
     for (int e = 0; e < 4; ++e)
-      if (q + e < nv) {
+      if (ALL || q + e < nv) {
         g[e] = sum_grad1<RB, GT>(t.g, R, i + e * STRIDE);
         w[e] = t.w[i + e * STRIDE];
-        m[e] = m_[e * STRIDE];
-        v[e] = v_[e * STRIDE];
+        m[e] = m_[im + e * STRIDE];
+        v[e] = v_[im + e * STRIDE];
       }
 #pragma unroll
     for (int e = 0; e < 4; ++e)
-      if (q + e < nv) {
+      if (ALL || q + e < nv) {
         update1(a, decay, __fmul_rn(g[e], s), w[e], m[e], v[e]);
-        m_[e * STRIDE] = m[e];
-        v_[e * STRIDE] = v[e];
+        m_[im + e * STRIDE] = m[e];
+        v_[im + e * STRIDE] = v[e];
         put_w1<RB>(t, R, a.lp_kind, i + e * STRIDE, w[e]);
       }
   }
 }
 
 // 8-bit state.  VEC: elements as in unit_vec, codes read and written four at a
-// time; else elements lane, lane + 32, ... below `avail`.
-template <int RB, typename GT, bool VEC>
-__device__ __forceinline__ void unit_quant(const View<RB> &t, const AdamWArgs &a, int R, float s,
-                                           float decay, size_t i, int avail, unsigned long long place,
-                                           unsigned char *m_, unsigned char *r_,
-                                           unsigned char *scale) {
+// time; else elements lane, lane + 32, ... below `avail` (ALL: it is 256).
+template <bool VEC> __device__ __forceinline__ int quant_at(int e) {
   const int lane = threadIdx.x & 31;
-  auto at = [&](int e) { return VEC ? 4 * lane + (e & 3) + 128 * (e >> 2) : lane + 32 * e; };
-  auto have = [&](int e) { return VEC || at(e) < avail; };
-  float g[8], w[8], m[8], r[8];
-  unsigned mc[4], rc[4];  // two codes each
-  const unsigned sc = *reinterpret_cast<const unsigned short *>(scale);
-  if constexpr (VEC) {
+  return VEC ? 4 * lane + (e & 3) + 128 * (e >> 2) : lane + 32 * e;
+}
+struct QuantUnit {      // what is read of a unit
+  float g[8], w[8];
+  unsigned m[2], r[2];  // four codes each, in the order of the elements
+  unsigned scale;
+};
+template <int RB, typename GT, bool VEC, bool ALL, typename Index>
+__device__ __forceinline__ void quant_load(QuantUnit &x, const View<RB> &t, int R, Index i, int avail,
+                                           const unsigned char *m_, const unsigned char *r_, Index im,
+                                           const unsigned char *scale) {
+  x.scale = *reinterpret_cast<const unsigned short *>(scale);
 #pragma unroll
-    for (int q = 0; q < 2; ++q) {
-      const int o = 4 * lane + 128 * q;
+  for (int q = 0; q < 2; ++q) {
+    if constexpr (VEC) {
+      const Index o = quant_at<true>(4 * q);
       float g4[4];
       sum_grad4<RB, GT>(t.g, R, i + o, g4);
-      const float4 w4 = *reinterpret_cast<const float4 *>(t.w + i + o);
-      const unsigned m4 = *reinterpret_cast<const unsigned *>(m_ + o);
-      const unsigned r4 = *reinterpret_cast<const unsigned *>(r_ + o);
-      mc[2 * q] = m4 & 0xffffu, mc[2 * q + 1] = m4 >> 16;
-      rc[2 * q] = r4 & 0xffffu, rc[2 * q + 1] = r4 >> 16;
+      const float4 w4 = *reinterpret_cast<const float4 *>(t.w + (i + o));
+      x.m[q] = *reinterpret_cast<const unsigned *>(m_ + (im + o));
+      x.r[q] = *reinterpret_cast<const unsigned *>(r_ + (im + o));
 #pragma unroll
-      for (int e = 0; e < 4; ++e) g[4 * q + e] = g4[e];
-      w[4 * q] = w4.x, w[4 * q + 1] = w4.y, w[4 * q + 2] = w4.z, w[4 * q + 3] = w4.w;
-    }
-  } else {
+      for (int e = 0; e < 4; ++e) x.g[4 * q + e] = g4[e];
+      x.w[4 * q] = w4.x, x.w[4 * q + 1] = w4.y, x.w[4 * q + 2] = w4.z, x.w[4 * q + 3] = w4.w;
+    } else {
+      unsigned cm[4], cr[4];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      g[e] = have(e) ? sum_grad1<RB, GT>(t.g, R, i + at(e)) : 0.f;
-      w[e] = have(e) ? t.w[i + at(e)] : 0.f;
-      const unsigned cm = have(e) ? m_[at(e)] : 0u, cr = have(e) ? r_[at(e)] : 0u;
-      mc[e >> 1] = e & 1 ? mc[e >> 1] | (cm << 8) : cm;
-      rc[e >> 1] = e & 1 ? rc[e >> 1] | (cr << 8) : cr;
+      for (int e = 0; e < 4; ++e) {
+        const Index o = quant_at<false>(4 * q + e);
+        const bool have = ALL || (int)o < avail;
+        x.g[4 * q + e] = have ? sum_grad1<RB, GT>(t.g, R, i + o) : 0.f;
+        x.w[4 * q + e] = have ? t.w[i + o] : 0.f;
+        cm[e] = have ? m_[im + o] : 0u, cr[e] = have ? r_[im + o] : 0u;
+      }
+      auto word = [](const unsigned (&c)[4]) {
+        return __byte_perm(__byte_perm(c[0], c[1], 0x0040), __byte_perm(c[2], c[3], 0x0040), 0x5410);
+      };
+      x.m[q] = word(cm), x.r[q] = word(cr);
     }
   }
-  const float m_scale = scale_of(sc & 0xffu), r_scale = scale_of(sc >> 8);
-  unsigned m_max = 0, r_max = 0;
+}
+// From what was read of a unit to its new weights (x.w, handed to put_w as soon as
+// they are there), codes and scale bytes.  Elements that do not exist are zeros in x.
+template <bool VEC, typename PutW>
+__device__ __forceinline__ void quant_step(QuantUnit &x, const AdamWArgs &a, float s, float decay,
+                                           unsigned long long place, PutW put_w) {
+  const float m_scale = scale_of(x.scale & 0xffu), r_scale = scale_of(x.scale >> 8);
+  float m[8], r[8];  // r: -v, then -sqrt(v)
+  float m_max = 0.f, v_max = 0.f;
+  unsigned low = 0xffffffffu;
 #pragma unroll
   for (int e = 0; e < 8; e += 2) {
-    Pair pm = mul2(decode2(mc[e >> 1]), twice(m_scale));
-    const Pair r0 = mul2(decode2(rc[e >> 1]), twice(r_scale));
-    const Pair pg = mul2(pair(g[e], g[e + 1]), twice(s));
-    pm = fma2(pm, twice(a.beta1), mul2(pg, twice(a.omb1)));
-    const Pair pr = root_near(fma2(mul2(r0, r0), twice(a.beta2), mul2(mul2(pg, pg), twice(a.omb2))));
-    unpair(step_w(a, decay, pair(w[e], w[e + 1]), pm, pr), w[e], w[e + 1]);
+    const int q = e >> 2, half = e & 2 ? 16 : 0;
+    Pair pm = mul2(decode2(x.m[q] >> half), twice(m_scale));
+    const Pair r0 = mul2(decode2(x.r[q] >> half), twice(r_scale));
+    const Pair g = mul2(pair(x.g[e], x.g[e + 1]), twice(s));
+    pm = fma2(pm, twice(a.beta1), mul2(g, twice(a.omb1)));
+    const Pair pv = fma2(mul2(r0, r0), twice(a.neg_beta2), mul2(mul2(g, g), twice(a.neg_omb2)));
     unpair(pm, m[e], m[e + 1]);
-    unpair(pr, r[e], r[e + 1]);
-#pragma unroll
-    for (int k = e; k < e + 2; ++k)
-      if (have(k)) {
-        m_max = max(m_max, __float_as_uint(m[k]) & 0x7fffffffu);
-        r_max = max(r_max, __float_as_uint(r[k]) & 0x7fffffffu);
-      }
+    unpair(pv, r[e], r[e + 1]);
+    // distance above -0, the smallest of those that are not 0
+    low = __vimin3_u32(low, __float_as_uint(r[e]) - 0x80000001u, __float_as_uint(r[e + 1]) - 0x80000001u);
+    m_max = max_abs(m_max, m[e], m[e + 1]);
+    v_max = max_abs(v_max, r[e], r[e + 1]);
   }
-  if constexpr (VEC) {
+  if (low < 0x0d800000u || !(v_max < __uint_as_float(0x7f800000u))) {  // some v below 2^-100, inf or nan
 #pragma unroll
-    for (int q = 0; q < 2; ++q) {
-      const float w4[4] = {w[4 * q], w[4 * q + 1], w[4 * q + 2], w[4 * q + 3]};
-      put_w4<RB>(t, R, a.lp_kind, i + 4 * lane + 128 * q, w4);
-    }
+    for (int e = 0; e < 8; ++e) r[e] = neg_root_any(r[e]);
   } else {
 #pragma unroll
-    for (int e = 0; e < 8; ++e)
-      if (have(e)) put_w1<RB>(t, R, a.lp_kind, i + at(e), w[e]);
+    for (int e = 0; e < 8; e += 2) unpair(neg_root(pair(r[e], r[e + 1])), r[e], r[e + 1]);
   }
-  const BlockScale mb = block_scale(__reduce_max_sync(0xffffffffu, m_max));
-  const BlockScale rb = block_scale(__reduce_max_sync(0xffffffffu, r_max));
+  float r_max = 0.f;
+#pragma unroll
+  for (int e = 0; e < 8; e += 2) {
+    float d0, d1;
+    unpair(fma2(pair(r[e], r[e + 1]), twice(a.neg_rs2), twice(a.eps)), d0, d1);
+    unpair(fma2(pair(x.w[e], x.w[e + 1]), twice(decay),
+                mul2(mul2(pair(m[e], m[e + 1]), twice(a.neg_c1)), pair(rcp_fast(d0), rcp_fast(d1)))),
+           x.w[e], x.w[e + 1]);
+    r_max = max_abs(r_max, r[e], r[e + 1]);
+  }
+  put_w();
+  const BlockScale mb = block_scale(__reduce_max_sync(0xffffffffu, __float_as_uint(m_max) & 0x7fffffffu));
+  const BlockScale rb = block_scale(__reduce_max_sync(0xffffffffu, __float_as_uint(r_max) & 0x7fffffffu));
+  x.scale = mb.byte | (rb.byte << 8);
   if (mb.big) {
 #pragma unroll
     for (int e = 0; e < 8; ++e) m[e] *= 0x1p-100f;
   }
   if (rb.big) {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) r[e] = r[e] > 0.f ? fmaxf(r[e] * 0x1p-100f, 0x1p-126f) : r[e];  // stays positive
+    for (int e = 0; e < 8; ++e) r[e] = r[e] < 0.f ? fminf(r[e] * 0x1p-100f, -0x1p-126f) : r[e];  // stays below 0
   }
   // place * multiplier + key, stepped from element to element
-  const unsigned first = (unsigned)(place + at(0)) * kPlaceMul + (unsigned)((place + at(0)) >> 32) * kHighMul + a.key;
-  unsigned cm[8], cr[8];
+  const unsigned long long p0 = place + quant_at<VEC>(0);
+  const unsigned first = (unsigned)p0 * kPlaceMul + (unsigned)(p0 >> 32) * kHighMul + a.key;
 #pragma unroll
-  for (int e = 0; e < 8; e += 2) {
-    float y[2], z[2];
-    unpair(mul2(pair(fabsf(m[e]), fabsf(m[e + 1])), twice(mb.factor)), y[0], y[1]);
-    unpair(mul2(pair(r[e], r[e + 1]), twice(rb.factor)), z[0], z[1]);
+  for (int q = 0; q < 2; ++q) {
+    unsigned cm[4], cr[4];
 #pragma unroll
-    for (int k = 0; k < 2; ++k) {
-      const unsigned bits = mix_bits(first + (unsigned)(at(e + k) - at(0)) * kPlaceMul);
-      cm[e + k] = encode(y[k], bits & 0xffffu) | ((__float_as_uint(m[e + k]) >> 24) & 0x80u);
-      const unsigned c = encode(z[k], bits >> 16);
-      cr[e + k] = r[e + k] > 0.f ? max(c, 1u) : c;
+    for (int e = 0; e < 4; e += 2) {
+      const int k = 4 * q + e;
+      float y[2], z[2];
+      unpair(mul2(pair(m[k], m[k + 1]), twice(mb.factor)), y[0], y[1]);
+      unpair(mul2(pair(r[k], r[k + 1]), twice(-rb.factor)), z[0], z[1]);
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const unsigned hash = mix_bits(first + (unsigned)(quant_at<VEC>(k + j) - quant_at<VEC>(0)) * kPlaceMul);
+        cm[e + j] = code_m(y[j], hash);
+        cr[e + j] = code_r(z[j], hash);
+      }
     }
-  }
-  if (mb.byte == 255u || rb.byte == 255u) {
+    unsigned mw = top_bytes(cm[0], cm[1], cm[2], cm[3]), rw = top_bytes(cr[0], cr[1], cr[2], cr[3]);
+    if (((rw + 0x7f7f7f7fu) & 0x80808080u) != 0x80808080u) {  // a root rounded to 0: 1 unless it is 0
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      if (mb.byte == 255u) cm[e] = 0u;
-      if (rb.byte == 255u) cr[e] = 0u;
+      for (int e = 0; e < 4; ++e)
+        if (r[4 * q + e] < 0.f && ((rw >> (8 * e)) & 0xffu) == 0u) rw |= 1u << (8 * e);
     }
+    x.m[q] = mb.byte == 255u ? 0u : mw;
+    x.r[q] = rb.byte == 255u ? 0u : rw;
   }
-  if constexpr (VEC) {
+}
+__device__ __forceinline__ void put_scale(const QuantUnit &x, unsigned char *scale) {
+  if ((threadIdx.x & 31) == 0) *reinterpret_cast<unsigned short *>(scale) = (unsigned short)x.scale;
+}
+template <int RB, typename GT, bool VEC, bool ALL, typename Index>
+__device__ __forceinline__ void unit_quant(const View<RB> &t, const AdamWArgs &a, int R, float s,
+                                           float decay, Index i, int avail, unsigned long long place,
+                                           unsigned char *m_, unsigned char *r_, Index im,
+                                           unsigned char *scale) {
+  QuantUnit x;
+  quant_load<RB, GT, VEC, ALL>(x, t, R, i, avail, m_, r_, im, scale);
+  quant_step<VEC>(x, a, s, decay, place, [&] {
 #pragma unroll
     for (int q = 0; q < 2; ++q) {
-      const int o = 4 * lane + 128 * q;
-      *reinterpret_cast<unsigned *>(m_ + o) =
-          cm[4 * q] | (cm[4 * q + 1] << 8) | (cm[4 * q + 2] << 16) | (cm[4 * q + 3] << 24);
-      *reinterpret_cast<unsigned *>(r_ + o) =
-          cr[4 * q] | (cr[4 * q + 1] << 8) | (cr[4 * q + 2] << 16) | (cr[4 * q + 3] << 24);
-    }
-  } else {
+      if constexpr (VEC) {
+        const float w4[4] = {x.w[4 * q], x.w[4 * q + 1], x.w[4 * q + 2], x.w[4 * q + 3]};
+        put_w4<RB>(t, R, a.lp_kind, i + (Index)quant_at<true>(4 * q), w4);
+      } else {
 #pragma unroll
-    for (int e = 0; e < 8; ++e)
-      if (have(e)) m_[at(e)] = (unsigned char)cm[e], r_[at(e)] = (unsigned char)cr[e];
+        for (int e = 4 * q; e < 4 * q + 4; ++e)
+          if (ALL || quant_at<false>(e) < avail) put_w1<RB>(t, R, a.lp_kind, i + (Index)quant_at<false>(e), x.w[e]);
+      }
+    }
+  });
+#pragma unroll
+  for (int q = 0; q < 2; ++q) {
+    if constexpr (VEC) {
+      *reinterpret_cast<unsigned *>(m_ + (im + quant_at<true>(4 * q))) = x.m[q];
+      *reinterpret_cast<unsigned *>(r_ + (im + quant_at<true>(4 * q))) = x.r[q];
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const Index o = quant_at<false>(4 * q + e);
+        if (ALL || (int)o < avail) m_[im + o] = (unsigned char)(x.m[q] >> (8 * e)), r_[im + o] = (unsigned char)(x.r[q] >> (8 * e));
+      }
+    }
   }
-  if (lane == 0) *reinterpret_cast<unsigned short *>(scale) = (unsigned short)(mb.byte | (rb.byte << 8));
+  put_scale(x, scale);
 }
 
 // A unit inside one tensor: `avail` (1..256) elements from element i of the
@@ -394,78 +474,334 @@ template <int RB, bool QUANT, typename GT>
 __device__ __forceinline__ void unit_inside(const View<RB> &t, const AdamWArgs &a, int R, float s,
                                             float decay, size_t i, int avail, bool vec, size_t e) {
   const int lane = threadIdx.x & 31;
+  const size_t im = e * kListGroup;
   if constexpr (QUANT) {
-    unsigned char *m = (unsigned char *)a.m + e * kListGroup, *r = (unsigned char *)a.v + e * kListGroup;
+    unsigned char *m = (unsigned char *)a.m, *r = (unsigned char *)a.v;
     unsigned char *scale = a.scale + e / kListUnitGroups * 2;
-    const unsigned long long place = a.flat0 + e * kListGroup;
     if (vec && avail == kListUnit)
-      unit_quant<RB, GT, true>(t, a, R, s, decay, i, avail, place, m, r, scale);
+      unit_quant<RB, GT, true, true>(t, a, R, s, decay, i, avail, a.flat0 + im, m, r, im, scale);
     else
-      unit_quant<RB, GT, false>(t, a, R, s, decay, i, avail, place, m, r, scale);
+      unit_quant<RB, GT, false, false>(t, a, R, s, decay, i, avail, a.flat0 + im, m, r, im, scale);
   } else {
-    float *m = (float *)a.m + e * kListGroup, *v = (float *)a.v + e * kListGroup;
+    float *m = (float *)a.m, *v = (float *)a.v;
     if (vec && avail == kListUnit)
-      unit_vec<RB, GT>(t, a, R, s, decay, i, m, v);
+      unit_vec<RB, GT>(t, a, R, s, decay, i, m, v, im);
     else
-      unit_scalar<RB, GT, 32>(t, a, R, s, decay, i + lane, avail > lane ? (avail - lane + 31) / 32 : 0,
-                              m + lane, v + lane);
+      unit_scalar<RB, GT, 32, false>(t, a, R, s, decay, i + lane, avail > lane ? (avail - lane + 31) / 32 : 0, m, v,
+                                     im + lane);
   }
 }
 
-// 16-byte accesses of fp32 weights and gradients, 8-byte ones of 16-bit types.
-template <typename GT> __device__ __forceinline__ bool vec_ok(const void *g, const float *w, const void *lp) {
-  return ((uintptr_t)g & (sizeof(GT) == 4 ? 15u : 7u)) == 0 && ((uintptr_t)w & 15u) == 0 &&
-         ((uintptr_t)lp & 7u) == 0;
+// ---- the kernels -----------------------------------------------------------------
+// Threads of a CTA and CTAs of an SM, fp32 moments.
+template <bool PACKED, typename GT> struct Shape {
+  static constexpr int kThreads = PACKED ? COCO_ADAMW_PACKED_THREADS
+                                  : sizeof(GT) == 4 ? COCO_ADAMW_THREADS32 : COCO_ADAMW_THREADS16;
+  static constexpr int kCtas = PACKED ? COCO_ADAMW_PACKED_CTAS
+                               : sizeof(GT) == 4 ? COCO_ADAMW_CTAS32 : COCO_ADAMW_CTAS16;
+};
+
+// A CTA's tile that holds several tensors or the end of one: every warp finds its
+// own unit.  Kept apart from the kernel's loop, whose registers decide its speed.
+template <bool QUANT, typename GT, int CAP>
+__device__ __noinline__ void tile_general(const ListTable<CAP> *tab, const AdamWArgs &a, const unsigned *s_off,
+                                          float s, unsigned tile) {
+  const int n = a.n, lane = threadIdx.x & 31;
+  const unsigned total = s_off[n];
+  const unsigned e = (tile * (blockDim.x >> 5) + (threadIdx.x >> 5)) * kListUnitGroups;
+  if (e >= total) return;
+  const int k = find_tensor(s_off, n, e);
+  const unsigned end = s_off[k + 1];
+  View<1> t;
+  if (QUANT || end - e >= kListUnitGroups || end == total) {
+    t.g[0] = tab->g[k], t.w = tab->w[k], t.lp = tab->lp[k];
+    const size_t left = (size_t)(end - e) * kListGroup - tab->missing[k];
+    unit_inside<1, QUANT, GT>(t, a, 1, s, tab->flags[k] & kListDecays ? a.decay : 1.f,
+                              (size_t)(e - s_off[k]) * kListGroup, left < kListUnit ? (int)left : kListUnit,
+                              (tab->flags[k] & kListAligned) != 0, e);
+  } else {
+    // several tensors in one unit: every lane looks up its own group
+    const unsigned el = e + lane;
+    if (el >= total) return;
+    const int kl = bisect(k, n - 1, el, [&](int x) { return s_off[x]; });
+    t.g[0] = tab->g[kl], t.w = tab->w[kl], t.lp = tab->lp[kl];
+    const int nv = el + 1 < s_off[kl + 1] ? kListGroup : kListGroup - tab->missing[kl];
+    const size_t im = (size_t)el * kListGroup;
+    unit_scalar<1, GT, 1, false>(t, a, 1, s, tab->flags[kl] & kListDecays ? a.decay : 1.f,
+                                 (size_t)(el - s_off[kl]) * kListGroup, nv, (float *)a.m, (float *)a.v, im);
+  }
 }
 
-// ---- the kernels -----------------------------------------------------------------
-template <bool QUANT, typename GT, int CAP>
-__global__ void __launch_bounds__(COCO_ADAMW_THREADS, 2)
+// A CTA takes tiles of one unit per warp.  Where a tile lies in one tensor, which and
+// where is the same for all threads: it costs no vector registers, and an element's
+// address is a common base and a 32-bit offset.  PACKED: such tiles have a form for
+// tensors that are not aligned, too.
+template <bool PACKED, typename GT, int CAP>
+__global__ void __launch_bounds__((Shape<PACKED, GT>::kThreads), (Shape<PACKED, GT>::kCtas))
     adamw_kernel(const __grid_constant__ ListTable<CAP> tab, const __grid_constant__ AdamWArgs a) {
   __shared__ unsigned s_off[CAP + 1];
-  for (int k = threadIdx.x; k <= a.n; k += blockDim.x) s_off[k] = tab.off[k];
+  const ListTable<CAP> *tp = &tab;
+  hide(tp);  // for lookups that differ from thread to thread
+  copy_offsets(s_off, tp->off, a.n);
   float s = a.grad_scale;
   if (a.norm) {
     if (!is_finite(a.norm[0])) return;  // the gradients are not usable: the step is skipped
     s = __fmul_rn(a.norm[1], s);
   }
   __syncthreads();
-  const int n = a.n, lane = threadIdx.x & 31;
-  const unsigned total = s_off[n];
-  const unsigned units = (total + kListUnitGroups - 1) / kListUnitGroups;
-  const unsigned nw = blockDim.x >> 5;
-  unsigned begin = 1, end = 0;  // the tensor at hand
-  unsigned missing = 0;
-  View<1> t = {};
-  float decay = 1.f;
-  bool vec = false;
-  for (unsigned u = blockIdx.x * nw + (threadIdx.x >> 5); u < units; u += gridDim.x * nw) {
-    const unsigned e = u * kListUnitGroups;
-    if (e < begin || e >= end) {
-      const int k = find_tensor(s_off, n, e);
-      begin = s_off[k], end = s_off[k + 1];
-      missing = tab.missing[k];
-      t.g[0] = tab.g[k], t.w = tab.w[k], t.lp = tab.lp[k];
-      decay = tab.decays[k] ? a.decay : 1.f;
-      vec = a.state_aligned && vec_ok<GT>(t.g[0], t.w, t.lp);
-    }
-    if (QUANT || end - e >= kListUnitGroups || end == total) {
-      const size_t left = (size_t)(end - e) * kListGroup - missing;
-      unit_inside<1, QUANT, GT>(t, a, 1, s, decay, (size_t)(e - begin) * kListGroup,
-                                left < kListUnit ? (int)left : kListUnit, vec, e);
+  constexpr unsigned kTile = Shape<PACKED, GT>::kThreads / 32 * kListUnitGroups;
+  const int n = a.n;
+  const unsigned tiles = (tab.off[n] + kTile - 1) / kTile;
+  const unsigned lane = threadIdx.x & 31, mine = (threadIdx.x & ~31u) * 8;  // elements before this warp's in the tile
+  int k = 0;  // the tensor in which the tile begins
+  for (unsigned tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
+    const unsigned e = tile * kTile;
+    int jump = 1;  // it lies at or behind the last one: double the steps, then halve them
+    while (k + jump < n && tab.off[k + jump] <= e) k += jump, jump *= 2;
+    for (; jump > 0; jump >>= 1)
+      if (k + jump < n && tab.off[k + jump] <= e) k += jump;
+    const unsigned end = tab.off[k + 1];
+    const bool aligned = (tab.flags[k] & kListAligned) != 0;
+    // the last group of a tensor may be short
+    if (e + kTile < end + (tab.missing[k] == 0) && (PACKED || aligned)) {
+      const size_t i = (size_t)(e - tab.off[k]) * kListGroup, im = (size_t)e * kListGroup;
+      View<1> t;
+      t.g[0] = (const GT *)tab.g[k] + i;
+      t.w = tab.w[k] + i;
+      t.lp = (unsigned short *)tab.lp[k] + i;
+      const float decay = tab.flags[k] & kListDecays ? a.decay : 1.f;
+      float *m = (float *)a.m + im, *v = (float *)a.v + im;
+      if (!PACKED || aligned)
+        unit_vec<1, GT>(t, a, 1, s, decay, mine, m, v, mine);
+      else
+        unit_scalar<1, GT, 32, true>(t, a, 1, s, decay, mine + lane, 8, m, v, mine + lane);
     } else {
-      // several tensors in one unit: every lane looks up its own group
-      const unsigned el = e + lane;
-      if (el < total) {
-        const int k = bisect(0, n - 1, el, [&](int x) { return s_off[x]; });
-        View<1> tl;
-        tl.g[0] = tab.g[k], tl.w = tab.w[k], tl.lp = tab.lp[k];
-        const int nv = el + 1 < s_off[k + 1] ? kListGroup : kListGroup - tab.missing[k];
-        unit_scalar<1, GT, 1>(tl, a, 1, s, tab.decays[k] ? a.decay : 1.f,
-                              (size_t)(el - s_off[k]) * kListGroup, nv,
-                              (float *)a.m + (size_t)el * kListGroup, (float *)a.v + (size_t)el * kListGroup);
+      tile_general<false, GT, CAP>(tp, a, s_off, s, tile);
+    }
+  }
+}
+
+// ---- 8-bit moments: tiles staged in shared memory ------------------------------------
+// The same walk with the loads in the hands of the copy engine: one thread asks for whole
+// tiles (bulk copies of the gradients, weights, codes and scales) two tiles ahead, so
+// that a warp finds its unit in shared memory and neither waits for HBM nor holds
+// registers for what is on its way.  A tile of a tensor that is not aligned is copied
+// from the 16-byte boundary below its start to the one above its end (memory of the same
+// allocation); its new weights leave through shared memory, in 16-byte stores but for
+// the ends of a unit.
+template <bool PACKED, typename GT> struct Pipe {
+  static constexpr int kThreads = COCO_ADAMW_QUANT_THREADS, kCtas = COCO_ADAMW_QUANT_CTAS;
+  static constexpr int kWarps = kThreads / 32, kTile = kWarps * kListUnit, kPad = PACKED ? 16 : 0;
+  static constexpr int kG = 0, kW = kG + kTile * (int)sizeof(GT) + kPad, kM = kW + kTile * 4 + kPad;
+  static constexpr int kR = kM + kTile, kScale = kR + kTile, kBytes = kScale + (kWarps * 2 + 15) / 16 * 16 + 16;
+  static constexpr int kLp = PACKED ? kWarps * (kListUnit * 2 + 16) : 0;  // copies on their way out
+  // of an SM's 228 KB: 1 KB per CTA is reserved, 5 KB are the kernel's other tables
+  static constexpr int kFit = ((228 * 1024) / kCtas - 6 * 1024 - kLp) / kBytes;
+  static constexpr int kStages = kFit < 3 ? kFit : 3;
+  static_assert(kStages >= 2 && kBytes % 16 == 0, "a tile is loaded while another is worked on");
+  static constexpr int kSmem = kStages * kBytes + kLp;
+};
+// The aligned 16-byte pieces that hold bytes [p, p + n).
+__device__ __forceinline__ unsigned window(const void *p, unsigned n) {
+  return ((unsigned)((uintptr_t)p & 15u) + n + 15u) & ~15u;
+}
+__device__ __forceinline__ const void *floor16(const void *p) { return (const void *)((uintptr_t)p & ~(uintptr_t)15u); }
+// n elements of T that lie in shared memory at the offset that p has within its 16
+// bytes, to p: whole 16-byte pieces at once, the ends one by one.
+template <typename T> __device__ __forceinline__ void store_window(T *p, const unsigned char *src, int n) {
+  constexpr int kN = 16 / (int)sizeof(T);
+  const int head = (int)((uintptr_t)p & 15u) / (int)sizeof(T);
+  T *first = p - head;
+  const T *from = reinterpret_cast<const T *>(src);
+  const int end = head + n;
+  for (int c = (threadIdx.x & 31) * kN; c < end; c += 32 * kN) {
+    if (c >= head && c + kN <= end) {
+      *reinterpret_cast<uint4 *>(first + c) = *reinterpret_cast<const uint4 *>(from + c);
+    } else {
+#pragma unroll
+      for (int j = 0; j < kN; ++j)
+        if (c + j >= head && c + j < end) first[c + j] = from[c + j];
+    }
+  }
+}
+
+// What the asker of a tile has found out about it, beside its data.
+struct TileInfo {
+  float *w;
+  unsigned short *lp;
+  int k;           // the tensor in which it begins
+  int staged;      // its data has been asked for: it lies in one tensor
+  float decay;
+  unsigned g_off;  // bytes between 16-byte boundaries and its gradients
+};
+
+template <bool PACKED, typename GT, int CAP>
+__global__ void __launch_bounds__((Pipe<PACKED, GT>::kThreads), (Pipe<PACKED, GT>::kCtas))
+    adamw8_kernel(const __grid_constant__ ListTable<CAP> tab, const __grid_constant__ AdamWArgs a) {
+  typedef Pipe<PACKED, GT> P;
+  constexpr unsigned S = P::kStages, kTileGroups = P::kTile / kListGroup;
+  extern __shared__ __align__(128) unsigned char s_stage[];
+  __shared__ unsigned s_off[CAP + 1];
+  __shared__ __align__(8) unsigned long long s_full[S], s_empty[S];
+  __shared__ __align__(16) TileInfo s_info[S];
+  const ListTable<CAP> *tp = &tab;
+  hide(tp);
+  copy_offsets(s_off, tp->off, a.n);
+  if (threadIdx.x == 0) {
+#pragma unroll
+    for (unsigned k = 0; k < S; ++k) mbar_init(&s_full[k], 1), mbar_init(&s_empty[k], P::kWarps);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  float s = a.grad_scale;
+  if (a.norm) {
+    if (!is_finite(a.norm[0])) return;  // the gradients are not usable: the step is skipped
+    s = __fmul_rn(a.norm[1], s);
+  }
+  __syncthreads();
+  const unsigned tiles = (s_off[a.n] + kTileGroups - 1) / kTileGroups;
+  const unsigned lane = threadIdx.x & 31, wid = threadIdx.x >> 5, mine = wid * kListUnit;
+
+  // Asks for a tile into a free stage; by one warp, k: a tensor at or before the tile's.
+  auto ask = [&](unsigned tile, unsigned st, int k) {
+    const unsigned e = tile * kTileGroups;
+    k += find_tensor(s_off + k, a.n - k, e);
+    if (lane == 0) {
+      const bool staged = e + kTileGroups < s_off[k + 1] + (tp->missing[k] == 0) &&  // its last group may be short
+                          (PACKED ? a.state_aligned != 0 : (tp->flags[k] & kListAligned) != 0);
+      const size_t i = (size_t)(e - s_off[k]) * kListGroup, im = (size_t)e * kListGroup;
+      const GT *g = (const GT *)tp->g[k] + i;
+      float *w = tp->w[k] + i;
+      TileInfo &info = s_info[st];
+      info.w = w, info.lp = (unsigned short *)tp->lp[k] + i;
+      info.k = k;
+      info.staged = staged;
+      info.decay = tp->flags[k] & kListDecays ? a.decay : 1.f;
+      info.g_off = (unsigned)((uintptr_t)g & 15u);
+      if (staged) {
+        unsigned char *dst = s_stage + st * P::kBytes;
+        const unsigned char *scale = a.scale + (size_t)tile * P::kWarps * 2;
+        const unsigned gb = window(g, P::kTile * (unsigned)sizeof(GT)), wb = window(w, P::kTile * 4);
+        const unsigned sb = window(scale, P::kWarps * 2);
+        mbar_expect_tx(&s_full[st], gb + wb + P::kTile * 2 + sb);
+        bulk_load(dst + P::kG, floor16(g), gb, &s_full[st]);
+        bulk_load(dst + P::kW, floor16(w), wb, &s_full[st]);
+        bulk_load(dst + P::kM, (const unsigned char *)a.m + im, P::kTile, &s_full[st]);
+        bulk_load(dst + P::kR, (const unsigned char *)a.v + im, P::kTile, &s_full[st]);
+        bulk_load(dst + P::kScale, floor16(scale), sb, &s_full[st]);
+      } else {
+        mbar_arrive(&s_full[st]);
       }
+    }
+    __syncwarp();
+  };
+
+  if (wid == 0)
+    for (unsigned d = 0; d < S - 1; ++d)
+      if (blockIdx.x + d * gridDim.x < tiles) ask(blockIdx.x + d * gridDim.x, d, 0);
+  unsigned st = 0, phase = 0, turn = 0;  // the stage at hand, its round, the warp whose turn it is to ask
+  bool ok = true;
+#pragma unroll 1
+  for (unsigned tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
+    ok = __all_sync(0xffffffffu, mbar_wait(&s_full[st], phase, a.timeout_ns));
+    if (!ok) break;
+    const TileInfo &info = s_info[st];
+    // the warps take turns at asking for the tile S - 1 ahead, into the stage that the
+    // tile before this one has left
+    if (turn == wid) {
+      const unsigned ahead = tile + (S - 1) * gridDim.x, to = st == 0 ? S - 1 : st - 1;
+      if (ahead < tiles) {
+        // the stage's first use needs no wait; its tile before was number j - 1 of this CTA
+        if (tile != blockIdx.x)
+          ok = __all_sync(0xffffffffu, mbar_wait(&s_empty[to], st == 0 ? phase ^ 1u : phase, a.timeout_ns));
+        if (!ok) break;
+        ask(ahead, to, info.k);
+      }
+    }
+    turn = turn + 1 == P::kWarps ? 0 : turn + 1;
+    if (info.staged) {
+      unsigned char *src = s_stage + st * P::kBytes;
+      const size_t im = (size_t)tile * P::kTile;
+      float *w = info.w + mine;
+      unsigned short *lp = info.lp + mine;
+      const float decay = info.decay;
+      const bool aligned = !PACKED || ((info.g_off | ((uintptr_t)w & 15u) | ((uintptr_t)lp & 15u)) == 0);
+      const unsigned char *gs = src + P::kG + (PACKED ? info.g_off : 0) + mine * sizeof(GT);
+      unsigned char *ws = src + P::kW + mine * 4;  // at a 16-byte boundary
+      const unsigned w_off = PACKED ? (unsigned)((uintptr_t)w & 15u) : 0;
+      QuantUnit x;
+#pragma unroll
+      for (int q = 0; q < 2; ++q) {
+        const unsigned o = 4 * lane + 128 * q;
+        float g4[4], w4[4];
+        if (aligned) {
+          widen4<GT>(*reinterpret_cast<const typename Raw<GT>::Four *>(gs + o * sizeof(GT)), g4);
+          widen4<float>(*reinterpret_cast<const uint4 *>(ws + o * 4), w4);
+        } else {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            g4[j] = Raw<GT>::widen1(reinterpret_cast<const typename Raw<GT>::One *>(gs)[o + j]);
+            w4[j] = reinterpret_cast<const float *>(ws + w_off)[o + j];
+          }
+        }
+        x.m[q] = *reinterpret_cast<const unsigned *>(src + P::kM + mine + o);
+        x.r[q] = *reinterpret_cast<const unsigned *>(src + P::kR + mine + o);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) x.g[4 * q + j] = g4[j], x.w[4 * q + j] = w4[j];
+      }
+      unsigned char *scale = a.scale + ((size_t)tile * P::kWarps + wid) * 2;
+      x.scale = *reinterpret_cast<const unsigned short *>(
+          src + P::kScale + ((uintptr_t)(a.scale + (size_t)tile * P::kWarps * 2) & 15u) + wid * 2);
       __syncwarp();
+      if (aligned && lane == 0) mbar_arrive(&s_empty[st]);
+      quant_step<true>(x, a, s, decay, a.flat0 + im + mine, [&] {
+        if (aligned) {
+          View<1> t;
+          t.w = w, t.lp = lp;
+#pragma unroll
+          for (int q = 0; q < 2; ++q) {
+            const float w4[4] = {x.w[4 * q], x.w[4 * q + 1], x.w[4 * q + 2], x.w[4 * q + 3]};
+            put_w4<1>(t, 1, a.lp_kind, 4 * lane + 128 * q, w4);
+          }
+          return;
+        }
+        unsigned char *ls = s_stage + S * P::kBytes + wid * (kListUnit * 2 + 16);
+        float *wo = reinterpret_cast<float *>(ws + w_off);
+        unsigned short *lo = reinterpret_cast<unsigned short *>(ls + ((uintptr_t)lp & 15u));
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          const unsigned o = quant_at<true>(k);
+          wo[o] = x.w[k];
+          if (a.lp_kind == kLpF16) lo[o] = Bits16<__half>::from_f32(x.w[k]);
+          else if (a.lp_kind == kLpBf16) lo[o] = Bits16<__nv_bfloat16>::from_f32(x.w[k]);
+        }
+        __syncwarp();
+        store_window(w, ws, kListUnit);
+        if (a.lp_kind != kLpNone) store_window(lp, ls, kListUnit);
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // before the next copy into this stage
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&s_empty[st]);
+      });
+      unsigned char *m = (unsigned char *)a.m + im, *r = (unsigned char *)a.v + im;
+#pragma unroll
+      for (int q = 0; q < 2; ++q) {
+        const unsigned o = mine + 4 * lane + 128 * q;
+        *reinterpret_cast<unsigned *>(m + o) = x.m[q];
+        *reinterpret_cast<unsigned *>(r + o) = x.r[q];
+      }
+      put_scale(x, scale);
+    } else {
+      if (lane == 0) mbar_arrive(&s_empty[st]);
+      tile_general<true, GT, CAP>(tp, a, s_off, s, tile);
+    }
+    if (++st == S) st = 0, phase ^= 1u;
+  }
+  if (!ok) {
+    // a copy or a warp of this CTA was not there in time: say so, and give the copies in
+    // flight one more bounded wait before the shared memory is given up
+    if (lane == 0) {
+      record_status(a.page, cocoTimeout, 0, kPhaseCopy, -1, 0);
+      for (unsigned d = 0; d < S; ++d, st = st + 1 == S ? 0 : st + 1, phase ^= st == 0)
+        mbar_wait(&s_full[st], phase, a.timeout_ns);
     }
   }
 }
@@ -505,10 +841,9 @@ __global__ void __launch_bounds__(COCO_ADAMW_PEER_THREADS, 2)
         const PeerPiece &pl = pieces[bisect(k, n - 1, el, [&](int x) { return pieces[x].off; })];
         const size_t done = (size_t)(el - pl.off) * kListGroup, left = (size_t)pl.len - done;
         const View<RB> t = {pl.g, pl.out, pl.w};
-        unit_scalar<RB, GT, 1>(t, a, R, s, pl.decays ? a.decay : 1.f, (size_t)pl.begin + done,
-                               left < kListGroup ? (int)left : kListGroup,
-                               (float *)a.m + (size_t)el * kListGroup,
-                               (float *)a.v + (size_t)el * kListGroup);
+        unit_scalar<RB, GT, 1, false>(t, a, R, s, pl.decays ? a.decay : 1.f, (size_t)pl.begin + done,
+                                      left < kListGroup ? (int)left : kListGroup, (float *)a.m, (float *)a.v,
+                                      (size_t)el * kListGroup);
       }
       __syncwarp();
     }
@@ -518,12 +853,30 @@ __global__ void __launch_bounds__(COCO_ADAMW_PEER_THREADS, 2)
 
 // ---- launches --------------------------------------------------------------------
 template <int CAP> using Kernel = void (*)(const ListTable<CAP>, const AdamWArgs);
-template <int CAP> Kernel<CAP> pick(bool quant, cocoDataType_t g) {
+struct LaunchShape {
+  int threads, ctas_per_sm, smem;
+};
+template <bool QUANT, bool PACKED, typename GT, int CAP> Kernel<CAP> pick_one(LaunchShape *sh) {
+  if constexpr (QUANT) {
+    typedef Pipe<PACKED, GT> P;
+    *sh = {P::kThreads, P::kCtas, P::kSmem};
+    return adamw8_kernel<PACKED, GT, CAP>;
+  } else {
+    typedef Shape<PACKED, GT> S;
+    *sh = {S::kThreads, S::kCtas, 0};
+    return adamw_kernel<PACKED, GT, CAP>;
+  }
+}
+template <int CAP> Kernel<CAP> pick(bool quant, bool packed, cocoDataType_t g, LaunchShape *sh) {
+  auto of = [&](auto type) -> Kernel<CAP> {
+    typedef decltype(type) GT;
+    return quant ? packed ? pick_one<true, true, GT, CAP>(sh) : pick_one<true, false, GT, CAP>(sh)
+           : packed ? pick_one<false, true, GT, CAP>(sh) : pick_one<false, false, GT, CAP>(sh);
+  };
   switch (g) {
-    case cocoFloat32: return quant ? adamw_kernel<true, float, CAP> : adamw_kernel<false, float, CAP>;
-    case cocoFloat16: return quant ? adamw_kernel<true, __half, CAP> : adamw_kernel<false, __half, CAP>;
-    case cocoBfloat16:
-      return quant ? adamw_kernel<true, __nv_bfloat16, CAP> : adamw_kernel<false, __nv_bfloat16, CAP>;
+    case cocoFloat32: return of(float());
+    case cocoFloat16: return of(__half());
+    case cocoBfloat16: return of(__nv_bfloat16());
   }
   return nullptr;
 }
@@ -549,21 +902,33 @@ unsigned adamw_rounding_key(uint64_t seed, int step) {
                   (unsigned)step * kPlaceMul);
 }
 
-int adamw_threads(bool, cocoDataType_t) { return COCO_ADAMW_THREADS; }
-int adamw_ctas_per_sm(bool, cocoDataType_t) { return 2; }
-
 template <int CAP>
-cudaError_t launch_adamw(bool quant, cocoDataType_t g_type, const ListTable<CAP> &table,
-                         const AdamWArgs &args, int ctas, cudaStream_t stream) {
-  const Kernel<CAP> k = pick<CAP>(quant, g_type);
+cudaError_t launch_adamw(bool quant, bool packed, cocoDataType_t g_type, const ListTable<CAP> &table,
+                         const AdamWArgs &args, size_t units, int device, int sm_count,
+                         int max_ctas_per_sm, cudaStream_t stream) {
+  LaunchShape sh;
+  const Kernel<CAP> k = pick<CAP>(quant, packed, g_type, &sh);
   if (!k) return cudaErrorInvalidValue;
+  if (sh.smem > 0) {  // more than the default: allowed once per kernel and device
+    static std::atomic<unsigned long long> allowed[2][3];
+    std::atomic<unsigned long long> &mask = allowed[packed][g_type == cocoFloat32 ? 0 : g_type == cocoFloat16 ? 1 : 2];
+    const unsigned long long bit = device < 64 ? 1ull << device : 0;
+    if (!(mask.load(std::memory_order_acquire) & bit)) {
+      const cudaError_t e = cudaFuncSetAttribute((const void *)k, cudaFuncAttributeMaxDynamicSharedMemorySize, sh.smem);
+      if (e != cudaSuccess) return e;
+      mask.fetch_or(bit, std::memory_order_release);
+    }
+  }
+  const int per_sm = max_ctas_per_sm > 0 && max_ctas_per_sm < sh.ctas_per_sm ? max_ctas_per_sm : sh.ctas_per_sm;
+  const size_t warps = (size_t)sh.threads / 32, need = (units + warps - 1) / warps, room = (size_t)per_sm * sm_count;
   void *params[] = {(void *)&table, (void *)&args};
-  return cudaLaunchKernel((const void *)k, dim3(ctas), dim3(COCO_ADAMW_THREADS), params, 0, stream);
+  return cudaLaunchKernel((const void *)k, dim3((unsigned)(need < room ? need : room)), dim3(sh.threads), params,
+                          sh.smem, stream);
 }
-template cudaError_t launch_adamw<kListCapSmall>(bool, cocoDataType_t, const ListTable<kListCapSmall> &,
-                                                 const AdamWArgs &, int, cudaStream_t);
-template cudaError_t launch_adamw<kListCapLarge>(bool, cocoDataType_t, const ListTable<kListCapLarge> &,
-                                                 const AdamWArgs &, int, cudaStream_t);
+template cudaError_t launch_adamw<kListCapSmall>(bool, bool, cocoDataType_t, const ListTable<kListCapSmall> &,
+                                                 const AdamWArgs &, size_t, int, int, int, cudaStream_t);
+template cudaError_t launch_adamw<kListCapLarge>(bool, bool, cocoDataType_t, const ListTable<kListCapLarge> &,
+                                                 const AdamWArgs &, size_t, int, int, int, cudaStream_t);
 
 cudaError_t launch_adamw_peers(bool quant, cocoDataType_t g_type, const PeerArgs &peers,
                                const AdamWArgs &args, const ListLaunch &cfg, cudaStream_t stream) {

@@ -1,6 +1,6 @@
 // Device helpers shared by the kernels that read and write peers' memory:
 // memory-model accesses, bounded waits and the status word, the exchange of
-// flags between ranks, 16-bit element types.
+// flags between ranks, mbarriers and bulk copies, 16-bit element types.
 #pragma once
 
 #include <cuda_bf16.h>
@@ -147,6 +147,59 @@ __device__ __forceinline__ int warp_wait_peers(const unsigned long long *slots, 
   if (p < R && p != rank) late = !wait_one(slots + p, seq, timeout_ns);
   const unsigned bad = __ballot_sync(0xffffffffu, late);
   return bad ? __ffs(bad) - 1 : -1;
+}
+
+// ---------------------------------------------------------------------------
+// mbarriers and bulk copies
+// ---------------------------------------------------------------------------
+__device__ __forceinline__ unsigned smem_u32(const void *p) {
+  return (unsigned)__cvta_generic_to_shared(p);
+}
+__device__ __forceinline__ void mbar_init(unsigned long long *bar, unsigned count) {
+  asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(bar)), "r"(count));
+}
+__device__ __forceinline__ void mbar_expect_tx(unsigned long long *bar, unsigned bytes) {
+  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(smem_u32(bar)),
+               "r"(bytes)
+               : "memory");
+}
+__device__ __forceinline__ void mbar_arrive(unsigned long long *bar) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+__device__ __forceinline__ bool mbar_try_wait(unsigned long long *bar, unsigned parity) {
+  unsigned ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(smem_u32(bar)), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
+// Bounded: gives up after timeout_ns (checked every 256 probes) or 2^26 probes.
+__device__ __noinline__ bool mbar_wait_slow(unsigned long long *bar, unsigned parity,
+                                            unsigned long long timeout_ns) {
+  const unsigned long long t0 = globaltimer_ns();
+  for (unsigned spin = 1; spin < (1u << 26); ++spin) {
+    if (mbar_try_wait(bar, parity)) return true;
+    if ((spin & 255u) == 0u && globaltimer_ns() - t0 > timeout_ns) return false;
+  }
+  return false;
+}
+__device__ __forceinline__ bool mbar_wait(unsigned long long *bar, unsigned parity,
+                                          unsigned long long timeout_ns) {
+  if (mbar_try_wait(bar, parity)) return true;
+  return mbar_wait_slow(bar, parity, timeout_ns);
+}
+// global -> shared bulk copy; src, dst and bytes are multiples of 16.
+__device__ __forceinline__ void bulk_load(void *dst, const void *src, unsigned bytes,
+                                          unsigned long long *bar) {
+  asm volatile(
+      "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::
+          "r"(smem_u32(dst)),
+      "l"(src), "r"(bytes), "r"(smem_u32(bar))
+      : "memory");
 }
 
 // ---------------------------------------------------------------------------

@@ -978,52 +978,6 @@ constexpr int kRingMaxStages = 4;
 constexpr int kRingMaxWarps = 16;
 constexpr unsigned kRingTileBytes = 512;  // 32 lanes x 16 bytes
 
-__device__ __forceinline__ unsigned smem_u32(const void *p) {
-  return (unsigned)__cvta_generic_to_shared(p);
-}
-__device__ __forceinline__ void mbar_init(unsigned long long *bar, unsigned count) {
-  asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(bar)), "r"(count));
-}
-__device__ __forceinline__ void mbar_expect_tx(unsigned long long *bar, unsigned bytes) {
-  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(smem_u32(bar)),
-               "r"(bytes)
-               : "memory");
-}
-__device__ __forceinline__ bool mbar_try_wait(unsigned long long *bar, unsigned parity) {
-  unsigned ok;
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
-      "selp.u32 %0, 1, 0, p;\n\t}"
-      : "=r"(ok)
-      : "r"(smem_u32(bar)), "r"(parity)
-      : "memory");
-  return ok != 0;
-}
-// Bounded: gives up after timeout_ns (checked every 256 probes) or 2^26 probes.
-__device__ __noinline__ bool mbar_wait_slow(unsigned long long *bar, unsigned parity,
-                                            unsigned long long timeout_ns) {
-  const unsigned long long t0 = globaltimer_ns();
-  for (unsigned spin = 1; spin < (1u << 26); ++spin) {
-    if (mbar_try_wait(bar, parity)) return true;
-    if ((spin & 255u) == 0u && globaltimer_ns() - t0 > timeout_ns) return false;
-  }
-  return false;
-}
-__device__ __forceinline__ bool mbar_wait(unsigned long long *bar, unsigned parity,
-                                          unsigned long long timeout_ns) {
-  if (mbar_try_wait(bar, parity)) return true;
-  return mbar_wait_slow(bar, parity, timeout_ns);
-}
-// global -> shared bulk copy; src, dst and bytes are multiples of 16.
-__device__ __forceinline__ void bulk_load(void *dst, const void *src, unsigned bytes,
-                                          unsigned long long *bar) {
-  asm volatile(
-      "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::
-          "r"(smem_u32(dst)),
-      "l"(src), "r"(bytes), "r"(smem_u32(bar))
-      : "memory");
-}
 __device__ __forceinline__ uint4 ld_shared_16(const void *p) {
   uint4 v;
   asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];"

@@ -13,6 +13,9 @@
 #ifndef COCO_NORM_THREADS
 #define COCO_NORM_THREADS 512
 #endif
+#ifndef COCO_NORM_CTAS
+#define COCO_NORM_CTAS 3
+#endif
 #ifndef COCO_NORM_DEPTH
 #define COCO_NORM_DEPTH 4
 #endif
@@ -59,15 +62,15 @@ template <typename GT> __device__ __forceinline__ double squares(const uint4 &q)
   if (s >= 0x1p-100f && s <= 0x1p126f) return (double)s;
   return squares_f64<GT>(q);
 }
-// 16 bytes of which only elements [a, b) exist: they are read one by one.
-template <typename GT>
-__device__ __forceinline__ double squares_part(const GT *p, int a, int b) {
-  double s = 0.0;
-  for (int e = a; e < b; ++e) {
-    const double x = (double)Raw<GT>::widen1(Raw<GT>::own1(p, e));
-    s += x * x;
-  }
-  return s;
+// The first `head` and last `tail` elements of 16 bytes replaced by zeros.
+template <typename GT> __device__ __forceinline__ uint4 masked(uint4 q, int head, int tail) {
+  constexpr int kN = Group<GT>::kN, kBits = 128 / kN;
+  unsigned w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+  for (int e = 0; e < kN; ++e)
+    if (e < head || e >= kN - tail)
+      w[e * kBits / 32] &= kBits == 32 ? 0u : e & 1 ? 0x0000ffffu : 0xffff0000u;
+  return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
 __device__ __forceinline__ double warp_sum(double x) {
@@ -117,58 +120,56 @@ __device__ __forceinline__ void put_norm(const NormArgs &a, float *out, double t
   out[1] = !is_finite(nf) ? 0.f : a.max_norm > 0.0 && n > a.max_norm ? (float)(a.max_norm / n) : 1.f;
 }
 
+// A tensor's first and last 16 bytes may hold elements of its neighbours: they are read
+// with it (16 aligned bytes that hold one of its elements are memory of the same
+// allocation) and masked.
 template <typename GT, int CAP>
-__global__ void __launch_bounds__(COCO_NORM_THREADS)
+__global__ void __launch_bounds__(COCO_NORM_THREADS, COCO_NORM_CTAS)
     norm_kernel(const __grid_constant__ NormTable<CAP> tab, const __grid_constant__ NormArgs a,
                 FlagPage *page) {
   __shared__ unsigned s_off[CAP + 1];
-  for (int k = threadIdx.x; k <= a.n; k += blockDim.x) s_off[k] = tab.off[k];
+  const NormTable<CAP> *tp = &tab;
+  hide(tp);  // for lookups that differ from lane to lane
+  copy_offsets(s_off, tp->off, a.n);
   __syncthreads();
   const int n = a.n, lane = threadIdx.x & 31;
   const unsigned total = s_off[n];
   const unsigned nw = blockDim.x >> 5;
-  constexpr int N = Group<GT>::kN;
-  unsigned begin = 1, end = 0, whole_a = 0, whole_b = 0;  // groups that exist as a whole
+  unsigned begin = 1, end = 0;  // the tensor at hand
   int head = 0, tail = 0;
   const uint4 *p = nullptr;
   double sum = 0.0;
-  auto enter = [&](unsigned e) {
-    const int k = find_tensor(s_off, n, e);
-    begin = s_off[k], end = s_off[k + 1];
-    p = (const uint4 *)tab.g[k];
-    head = tab.head[k], tail = tab.tail[k];
-    whole_a = begin + (head ? 1 : 0), whole_b = end - (tail ? 1 : 0);
-  };
-  // one group of a tensor that may be cut at its ends
-  auto edge = [&](const uint4 *q, unsigned x, unsigned b, unsigned z, int h, int t) {
-    return squares_part<GT>((const GT *)(q + (x - b)), x == b ? h : 0, x == z - 1 ? N - t : N);
-  };
   for (unsigned u = blockIdx.x * nw + (threadIdx.x >> 5); u < (total + kUnit - 1) / kUnit;
        u += gridDim.x * nw) {
     const unsigned e = u * kUnit;
-    if (e < begin || e >= end) enter(e);
-    if (e >= whole_a && e + kUnit <= whole_b) {
-      uint4 q[kDepth];
+    if (e < begin || e >= end) {
+      const int k = find_tensor(s_off, n, e);
+      begin = s_off[k], end = s_off[k + 1];
+      p = (const uint4 *)tab.g[k];
+      head = tab.head[k], tail = tab.tail[k];
+    }
+    uint4 q[kDepth];
+    if (e + kUnit <= end) {
 #pragma unroll
       for (int k = 0; k < kDepth; ++k) q[k] = p[e - begin + lane + 32 * k];
+      if (head && e == begin && lane == 0) q[0] = masked<GT>(q[0], head, 0);
+      if (tail && e + kUnit == end && lane == 31) q[kDepth - 1] = masked<GT>(q[kDepth - 1], 0, tail);
+    } else {  // several tensors: every group looks up its own
 #pragma unroll
-      for (int k = 0; k < kDepth; ++k) sum += squares<GT>(q[k]);
-      continue;
-    }
-#pragma unroll 1
-    for (int k = 0; k < kDepth; ++k) {
-      const unsigned ek = e + 32 * k, x = ek + lane;
-      if (ek >= total) break;
-      if (ek < begin || ek >= end) enter(ek);
-      if (ek + 32 <= end || end == total) {
-        if (x >= whole_a && x < whole_b) sum += squares<GT>(p[x - begin]);
-        else if (x < end) sum += edge(p, x, begin, end, head, tail);
-      } else if (x < total) {
-        const int t = bisect(0, n - 1, x, [&](int y) { return s_off[y]; });
-        sum += edge((const uint4 *)tab.g[t], x, s_off[t], s_off[t + 1], tab.head[t], tab.tail[t]);
+      for (int k = 0; k < kDepth; ++k) {
+        const unsigned x = e + lane + 32 * k;
+        q[k] = make_uint4(0u, 0u, 0u, 0u);
+        if (x < total) {
+          const int t = bisect(0, n - 1, x, [&](int y) { return s_off[y]; });
+          q[k] = ((const uint4 *)tp->g[t])[x - s_off[t]];
+          const int h = x == s_off[t] ? tp->head[t] : 0, l = x == s_off[t + 1] - 1 ? tp->tail[t] : 0;
+          if (h | l) q[k] = masked<GT>(q[k], h, l);
+        }
       }
       __syncwarp();
     }
+#pragma unroll
+    for (int k = 0; k < kDepth; ++k) sum += squares<GT>(q[k]);
   }
   double all = 0.0;
   if (!rank_sum(sum, page, all) || threadIdx.x != 0) return;
@@ -268,6 +269,7 @@ PeerKernel pick_peer(cocoDataType_t g, int world) {
 }  // namespace
 
 int grad_norm_threads() { return COCO_NORM_THREADS; }
+int grad_norm_ctas_per_sm() { return COCO_NORM_CTAS; }
 int grad_norm_groups_per_warp() { return kUnit; }
 
 template <int CAP>

@@ -24,16 +24,16 @@ template <typename GT> __device__ __forceinline__ void widen4(uint2 q, float (&x
 template <typename GT> struct Raw {
   typedef uint2 Four;
   typedef unsigned short One;
-  static __device__ __forceinline__ Four peer4(const void *p, size_t i) {
+  template <typename Index> static __device__ __forceinline__ Four peer4(const void *p, Index i) {
     return ld_sys_8((const unsigned short *)p + i);
   }
-  static __device__ __forceinline__ One peer1(const void *p, size_t i) {
+  template <typename Index> static __device__ __forceinline__ One peer1(const void *p, Index i) {
     return ld_sys_2((const unsigned short *)p + i);
   }
-  static __device__ __forceinline__ Four own4(const void *p, size_t i) {
+  template <typename Index> static __device__ __forceinline__ Four own4(const void *p, Index i) {
     return *reinterpret_cast<const uint2 *>((const unsigned short *)p + i);
   }
-  static __device__ __forceinline__ One own1(const void *p, size_t i) {
+  template <typename Index> static __device__ __forceinline__ One own1(const void *p, Index i) {
     return ((const unsigned short *)p)[i];
   }
   static __device__ __forceinline__ float widen1(One b) { return Bits16<GT>::to_f32(b); }
@@ -41,23 +41,23 @@ template <typename GT> struct Raw {
 template <> struct Raw<float> {
   typedef uint4 Four;
   typedef unsigned One;
-  static __device__ __forceinline__ Four peer4(const void *p, size_t i) {
+  template <typename Index> static __device__ __forceinline__ Four peer4(const void *p, Index i) {
     return ld_sys_16((const float *)p + i);
   }
-  static __device__ __forceinline__ One peer1(const void *p, size_t i) {
+  template <typename Index> static __device__ __forceinline__ One peer1(const void *p, Index i) {
     return ld_sys_4((const float *)p + i);
   }
-  static __device__ __forceinline__ Four own4(const void *p, size_t i) {
+  template <typename Index> static __device__ __forceinline__ Four own4(const void *p, Index i) {
     return *reinterpret_cast<const uint4 *>((const float *)p + i);
   }
-  static __device__ __forceinline__ One own1(const void *p, size_t i) {
+  template <typename Index> static __device__ __forceinline__ One own1(const void *p, Index i) {
     return ((const unsigned *)p)[i];
   }
   static __device__ __forceinline__ float widen1(One b) { return __uint_as_float(b); }
 };
 
-template <int RB, typename GT>
-__device__ __forceinline__ void sum_grad4(const void *const *g, int R, size_t i, float (&x)[4]) {
+template <int RB, typename GT, typename Index>
+__device__ __forceinline__ void sum_grad4(const void *const *g, int R, Index i, float (&x)[4]) {
   if constexpr (RB == 1) {
     widen4<GT>(Raw<GT>::own4(g[0], i), x);
   } else {
@@ -76,8 +76,8 @@ __device__ __forceinline__ void sum_grad4(const void *const *g, int R, size_t i,
       }
   }
 }
-template <int RB, typename GT>
-__device__ __forceinline__ float sum_grad1(const void *const *g, int R, size_t i) {
+template <int RB, typename GT, typename Index>
+__device__ __forceinline__ float sum_grad1(const void *const *g, int R, Index i) {
   if constexpr (RB == 1) {
     return Raw<GT>::widen1(Raw<GT>::own1(g[0], i));
   } else {
@@ -130,6 +130,14 @@ __device__ __forceinline__ void list_end_barrier(const PeerRank &pr, const PeerA
   const int late = warp_wait_peers(me->done, pa.world, pr.rank, pa.seq, pa.timeout_ns);
   if (late >= 0 && threadIdx.x == 0)
     record_status(me, cocoTimeout, pr.rank, kPhaseEnd, late, pa.seq);
+}
+
+// Makes the compiler forget that a pointer is to a kernel parameter: reads of the
+// constant bank at 32 different places take turns, through a plain pointer they are
+// one access per warp.
+template <typename T> __device__ __forceinline__ void hide(const T *&p) { asm volatile("" : "+l"(p)); }
+__device__ __forceinline__ void copy_offsets(unsigned *dst, const unsigned *off, int n) {
+  for (int k = threadIdx.x; k <= n; k += blockDim.x) dst[k] = off[k];
 }
 
 // ---- finding a tensor ----------------------------------------------------------

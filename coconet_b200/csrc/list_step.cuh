@@ -31,9 +31,11 @@ template <int CAP> struct ListTable {
   void *lp[CAP];
   unsigned off[CAP + 1];         // tensor's first group; [n]: one past the last
   unsigned char missing[CAP];    // elements of the tensor's groups that do not exist
-  unsigned char decays[CAP];     // weight decay applies
+  unsigned char flags[CAP];      // kListDecays, kListAligned
 };
 
+// weight decay applies; gradient, weights and copy start on 16 bytes and so does the state
+enum : unsigned char { kListDecays = 1, kListAligned = 2 };
 enum : int { kLpNone = 0, kLpF16 = 1, kLpBf16 = 2 };
 enum : int { kListAdamW = 1, kListAdamWQuant = 2, kListGradNorm = 3 };  // operations on lists
 
@@ -42,13 +44,16 @@ struct AdamWArgs {
   unsigned char *scale;          // 8-bit state: two bytes per block
   const float *norm;             // {gradient norm, clip factor} or null
   unsigned long long flat0;      // place of that state in the flat state of the whole list
+  FlagPage *page;                // world size 1: whose status word a copy that does not land is written to,
+  unsigned long long timeout_ns; // after this time
   int n;                         // tensors in the table (world size 1)
   int lp_kind;
-  int state_aligned;             // m and v (codes) allow the vector path
+  int state_aligned;             // m and v start on 16 bytes
   unsigned key;                  // of the rounding bits
   float grad_scale, beta1, beta2, omb1, omb2;
   float neg_c1;                  // -lr / (1 - beta1^t)
   float rs2;                     // 1 / sqrt(1 - beta2^t)
+  float neg_beta2, neg_omb2, neg_rs2;
   float eps, decay;              // decay: 1 - lr * weight_decay
 };
 
@@ -80,8 +85,7 @@ struct PeerArgs {
 };
 
 // Gradient norm, world size 1: counted in groups of 16 bytes.  A tensor whose
-// start is not 16-byte aligned is walked from the aligned address below it;
-// the elements outside are not read.
+// start is not 16-byte aligned is walked from the aligned address below it.
 constexpr int kNormCapSmall = 64, kNormCapLarge = 1024;
 template <int CAP> struct NormTable {
   const void *g[CAP];                  // rounded down to 16 bytes
@@ -101,13 +105,13 @@ struct ListLaunch {
   bool cooperative;
 };
 
-// cudaErrorInvalidValue for a type that has no kernel.
+// cudaErrorInvalidValue for a type that has no kernel.  packed: tensors of 256
+// elements or more are not all aligned (aligned16), or the state is not.
 template <int CAP>
-cudaError_t launch_adamw(bool quant, cocoDataType_t g_type, const ListTable<CAP> &table,
-                         const AdamWArgs &args, int ctas, cudaStream_t stream);
+cudaError_t launch_adamw(bool quant, bool packed, cocoDataType_t g_type, const ListTable<CAP> &table,
+                         const AdamWArgs &args, size_t units, int device, int sm_count,
+                         int max_ctas_per_sm, cudaStream_t stream);
 unsigned adamw_rounding_key(uint64_t seed, int step);
-int adamw_threads(bool quant, cocoDataType_t g_type);
-int adamw_ctas_per_sm(bool quant, cocoDataType_t g_type);
 cudaError_t launch_adamw_peers(bool quant, cocoDataType_t g_type, const PeerArgs &peers,
                                const AdamWArgs &args, const ListLaunch &cfg, cudaStream_t stream);
 cudaError_t adamw_peers_occupancy(bool quant, cocoDataType_t g_type, int world, int threads,
@@ -117,6 +121,7 @@ template <int CAP>
 cudaError_t launch_grad_norm(cocoDataType_t g_type, const NormTable<CAP> &table,
                              const NormArgs &args, FlagPage *page, int ctas, cudaStream_t stream);
 int grad_norm_threads();
+int grad_norm_ctas_per_sm();
 int grad_norm_groups_per_warp();  // 16-byte groups a warp takes per pass
 cudaError_t launch_grad_norm_peers(cocoDataType_t g_type, const PeerArgs &peers,
                                    const NormArgs &args, const ListLaunch &cfg,

@@ -874,14 +874,16 @@ template <int CAP> int launch_adamw_local(cocoComm *c, const ListCall &lc) {
   const bool quant = lc.op == kListAdamWQuant;
   const size_t align_groups = list_align(lc.op) / kListGroup;
   const size_t state_bytes = quant ? 1 : sizeof(float);
-  const int threads = adamw_threads(quant, lc.g_type), per_sm = adamw_ctas_per_sm(quant, lc.g_type);
   static thread_local ListTable<CAP> tab;
   AdamWArgs a = lc.adam;
+  a.page = c->flags;
+  a.timeout_ns = (unsigned long long)c->timeout_ms * 1000000ull;
   size_t groups_before = 0;
   size_t b = 0;
   while (b < lc.n) {
     int n = 0;
     size_t at = 0;
+    bool packed = false;
     for (; b < lc.n && n < CAP; ++b) {
       const size_t count = lc.counts[b];
       if (count == 0) continue;
@@ -892,7 +894,9 @@ template <int CAP> int launch_adamw_local(cocoComm *c, const ListCall &lc) {
       tab.lp[n] = lc.lp ? lc.lp[b] : nullptr;
       tab.off[n] = (unsigned)at;
       tab.missing[n] = (unsigned char)(len * kListGroup - count);
-      tab.decays[n] = !(lc.no_decay && lc.no_decay[b]);
+      const bool aligned = a.state_aligned && aligned16(lc.g[b]) && aligned16(lc.w[b]) && aligned16(tab.lp[n]);
+      tab.flags[n] = (lc.no_decay && lc.no_decay[b] ? 0 : kListDecays) | (aligned ? kListAligned : 0);
+      packed = packed || (count >= (size_t)kListUnit && !aligned);
       at += len;
       ++n;
     }
@@ -904,7 +908,8 @@ template <int CAP> int launch_adamw_local(cocoComm *c, const ListCall &lc) {
     a.scale = quant ? lc.adam.scale + groups_before / kListUnitGroups * 2 : nullptr;
     a.flat0 = groups_before * kListGroup;
     const size_t units = (at + kListUnitGroups - 1) / kListUnitGroups;
-    CUDA_TRY(launch_adamw<CAP>(quant, lc.g_type, tab, a, ctas_for(c, units, threads, per_sm), lc.stream));
+    CUDA_TRY(launch_adamw<CAP>(quant, packed, lc.g_type, tab, a, units, c->device, c->sm_count,
+                               c->ctas_per_sm, lc.stream));
     c->launches++;
     groups_before += at;
   }
@@ -944,7 +949,7 @@ template <int CAP> int launch_norm_local(cocoComm *c, const ListCall &lc) {
     a.n = n;
     a.last = b >= lc.n;
     const size_t units = (at + grad_norm_groups_per_warp() - 1) / grad_norm_groups_per_warp();
-    CUDA_TRY(launch_grad_norm<CAP>(lc.g_type, tab, a, c->flags, ctas_for(c, units, grad_norm_threads(), 2),
+    CUDA_TRY(launch_grad_norm<CAP>(lc.g_type, tab, a, c->flags, ctas_for(c, units, grad_norm_threads(), grad_norm_ctas_per_sm()),
                                    lc.stream));
     c->launches++;
     a.first = 0;
@@ -1136,8 +1141,7 @@ int enqueue_list_or_throw(cocoComm *c, ListCall &lc) {
   COCO_TRY(validate_list(c, lc, &total));
   if (total == 0 && lc.op != kListGradNorm) return cocoSuccess;
   if (lc.op != kListGradNorm) {
-    const uintptr_t mask = lc.op == kListAdamWQuant ? 3u : 15u;
-    lc.adam.state_aligned = (((uintptr_t)lc.adam.m | (uintptr_t)lc.adam.v) & mask) == 0;
+    lc.adam.state_aligned = (((uintptr_t)lc.adam.m | (uintptr_t)lc.adam.v) & 15u) == 0;
     lc.adam.lp_kind = !lc.lp ? kLpNone : lc.lp_type == cocoFloat16 ? kLpF16 : kLpBf16;
   }
   NvtxRange range(lc.op == kListGradNorm ? "coconet gradient norm" : "coconet fused AdamW");
@@ -1974,6 +1978,7 @@ static int adamw_call(ListCall *lc, cocoComm_t comm, size_t nbuff, const void *c
   a.omb1 = 1.0f - beta1, a.omb2 = 1.0f - beta2;
   a.neg_c1 = (float)(-(double)lr / d1);
   a.rs2 = (float)(1.0 / std::sqrt(d2));
+  a.neg_beta2 = -a.beta2, a.neg_omb2 = -a.omb2, a.neg_rs2 = -a.rs2;
   a.eps = eps;
   a.decay = (float)(1.0 - (double)lr * (double)weight_decay);
   lc->stream = (cudaStream_t)stream;

@@ -334,7 +334,7 @@ class TensorList:
 
     def _checked(self, weights):
         """Types, sizes and devices of the list, looked over at its first use by
-        the gradient norm or an AdamW call.  Returns the device."""
+        the gradient norm or an AdamW call.  Returns the device's number."""
         gs, ws, lps = self.tensors
         if weights and ws is None:
             raise ValueError("this list holds no weights")
@@ -355,7 +355,7 @@ class TensorList:
                         raise ValueError(f"{what} {k} holds {t.numel()} elements, not {count}")
             if lps and lps[0].dtype not in (torch.float16, torch.bfloat16):
                 raise ValueError(f"low-precision copies are fp16 or bf16, not {lps[0].dtype}")
-            self._device = dev
+            self._device = index
         return self._device
 
     def _slice(self, world, quant):
@@ -379,6 +379,7 @@ class Communicator:
         self._h = C.c_void_p(handle)
         self.world = world
         self.rank = rank
+        self._device = None   # looked up by the first call that compares it
 
     # ---- construction ----
     @classmethod
@@ -540,20 +541,20 @@ class Communicator:
         """The stream to use: `stream`, or the current one of the list's device,
         which has to be this communicator's."""
         import torch
-        if getattr(self, "_device", None) is None:
+        if self._device is None:
             d = C.c_int()
             _check(lib().cocoCommCuDevice(self._h, C.byref(d)), "cocoCommCuDevice")
             self._device = d.value
-        if device.index != self._device:
-            raise ValueError(f"the tensors are on {device}, the communicator on cuda:{self._device}")
-        return C.c_void_p((stream if stream is not None else torch.cuda.current_stream(device)).cuda_stream)
+        if device != self._device:
+            raise ValueError(f"the tensors are on cuda:{device}, the communicator on cuda:{self._device}")
+        return stream.cuda_stream if stream is not None else torch._C._cuda_getCurrentRawStream(device)
 
     @staticmethod
     def _held(t, what, device, dtypes, least):
         """Pointer of a state tensor after a look at its type and size."""
-        if t.dtype not in dtypes or t.device != device or not t.is_contiguous() or t.numel() < least:
+        if t.dtype not in dtypes or t.get_device() != device or not t.is_contiguous() or t.numel() < least:
             raise ValueError(f"{what}: at least {least} contiguous elements of {' or '.join(map(str, dtypes))} on "
-                             f"{device} are needed, got {tuple(t.shape)} {t.dtype} on {t.device}")
+                             f"cuda:{device} are needed, got {tuple(t.shape)} {t.dtype} on {t.device}")
         return t.data_ptr()
 
     def grad_norm_scattered(self, gs, norm, max_norm=0.0, grad_scale=1.0, stream=None):
