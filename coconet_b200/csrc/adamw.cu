@@ -23,29 +23,18 @@
 
 #include <atomic>
 
-#ifndef COCO_ADAMW_THREADS16
-#define COCO_ADAMW_THREADS16 352
-#endif
-#ifndef COCO_ADAMW_CTAS16
-#define COCO_ADAMW_CTAS16 2
-#endif
-#ifndef COCO_ADAMW_THREADS32
-#define COCO_ADAMW_THREADS32 352
-#endif
-#ifndef COCO_ADAMW_CTAS32
-#define COCO_ADAMW_CTAS32 2
+// Threads of a CTA, two CTAs per SM, and tiles in flight of the staged kernels.
+#ifndef COCO_ADAMW_THREADS
+#define COCO_ADAMW_THREADS 352
 #endif
 #ifndef COCO_ADAMW_PACKED_THREADS
-#define COCO_ADAMW_PACKED_THREADS 512
-#endif
-#ifndef COCO_ADAMW_PACKED_CTAS
-#define COCO_ADAMW_PACKED_CTAS 2
+#define COCO_ADAMW_PACKED_THREADS 256
 #endif
 #ifndef COCO_ADAMW_QUANT_THREADS
-#define COCO_ADAMW_QUANT_THREADS 512
+#define COCO_ADAMW_QUANT_THREADS 384
 #endif
-#ifndef COCO_ADAMW_QUANT_CTAS
-#define COCO_ADAMW_QUANT_CTAS 2
+#ifndef COCO_ADAMW_STAGES
+#define COCO_ADAMW_STAGES 3
 #endif
 #ifndef COCO_ADAMW_PEER_THREADS
 #define COCO_ADAMW_PEER_THREADS 256
@@ -66,16 +55,20 @@ template <> struct View<1> {
   void *lp;
 };
 
+// Two values as 16-bit numbers in one word.
+__device__ __forceinline__ unsigned lp_pair(int kind, float x, float y) {
+  if (kind == kLpF16) {
+    const __half2 h = __floats2half2_rn(x, y);
+    return *reinterpret_cast<const unsigned *>(&h);
+  }
+  const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
+  return *reinterpret_cast<const unsigned *>(&h);
+}
 template <int RB, typename Index> __device__ __forceinline__ void put_lp4(const View<RB> &v, int R, int kind, Index i,
                                                           const float (&x)[4]) {
   uint2 q;
-  if (kind == kLpF16) {
-    const __half2 a = __floats2half2_rn(x[0], x[1]), b = __floats2half2_rn(x[2], x[3]);
-    q = make_uint2(*reinterpret_cast<const unsigned *>(&a), *reinterpret_cast<const unsigned *>(&b));
-  } else {
-    const __nv_bfloat162 a = __floats2bfloat162_rn(x[0], x[1]), b = __floats2bfloat162_rn(x[2], x[3]);
-    q = make_uint2(*reinterpret_cast<const unsigned *>(&a), *reinterpret_cast<const unsigned *>(&b));
-  }
+  if (kind == kLpF16) q = make_uint2(lp_pair(kLpF16, x[0], x[1]), lp_pair(kLpF16, x[2], x[3]));
+  else q = make_uint2(lp_pair(kLpBf16, x[0], x[1]), lp_pair(kLpBf16, x[2], x[3]));
   if constexpr (RB == 1) {
     *reinterpret_cast<uint2 *>((unsigned short *)v.lp + i) = q;
   } else {
@@ -276,16 +269,16 @@ __device__ __forceinline__ void unit_vec(const View<RB> &t, const AdamWArgs &a, 
     put_w4<RB>(t, R, a.lp_kind, i + o, w4);
   }
 }
-// Scalar form: nv (0..8) elements of this lane, STRIDE apart, four at a time; ALL: eight.
-template <int RB, typename GT, int STRIDE, bool ALL, typename Index>
+// Scalar form: nv (0..8) elements of this lane, STRIDE apart, four at a time.
+template <int RB, typename GT, int STRIDE, typename Index>
 __device__ __forceinline__ void unit_scalar(const View<RB> &t, const AdamWArgs &a, int R, float s,
                                             float decay, Index i, int nv, float *m_, float *v_, Index im) {
 #pragma unroll 1
-  for (int q = 0; q < (ALL ? 8 : nv); q += 4, i += 4 * STRIDE, im += 4 * STRIDE) {
+  for (int q = 0; q < nv; q += 4, i += 4 * STRIDE, im += 4 * STRIDE) {
     float g[4], w[4], m[4], v[4];
 #pragma unroll
     for (int e = 0; e < 4; ++e)
-      if (ALL || q + e < nv) {
+      if (q + e < nv) {
         g[e] = sum_grad1<RB, GT>(t.g, R, i + e * STRIDE);
         w[e] = t.w[i + e * STRIDE];
         m[e] = m_[im + e * STRIDE];
@@ -293,7 +286,7 @@ __device__ __forceinline__ void unit_scalar(const View<RB> &t, const AdamWArgs &
       }
 #pragma unroll
     for (int e = 0; e < 4; ++e)
-      if (ALL || q + e < nv) {
+      if (q + e < nv) {
         update1(a, decay, __fmul_rn(g[e], s), w[e], m[e], v[e]);
         m_[im + e * STRIDE] = m[e];
         v_[im + e * STRIDE] = v[e];
@@ -303,7 +296,7 @@ __device__ __forceinline__ void unit_scalar(const View<RB> &t, const AdamWArgs &
 }
 
 // 8-bit state.  VEC: elements as in unit_vec, codes read and written four at a
-// time; else elements lane, lane + 32, ... below `avail` (ALL: it is 256).
+// time; else elements lane, lane + 32, ... below `avail`.
 template <bool VEC> __device__ __forceinline__ int quant_at(int e) {
   const int lane = threadIdx.x & 31;
   return VEC ? 4 * lane + (e & 3) + 128 * (e >> 2) : lane + 32 * e;
@@ -313,7 +306,7 @@ struct QuantUnit {      // what is read of a unit
   unsigned m[2], r[2];  // four codes each, in the order of the elements
   unsigned scale;
 };
-template <int RB, typename GT, bool VEC, bool ALL, typename Index>
+template <int RB, typename GT, bool VEC, typename Index>
 __device__ __forceinline__ void quant_load(QuantUnit &x, const View<RB> &t, int R, Index i, int avail,
                                            const unsigned char *m_, const unsigned char *r_, Index im,
                                            const unsigned char *scale) {
@@ -335,7 +328,7 @@ __device__ __forceinline__ void quant_load(QuantUnit &x, const View<RB> &t, int 
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const Index o = quant_at<false>(4 * q + e);
-        const bool have = ALL || (int)o < avail;
+        const bool have = (int)o < avail;
         x.g[4 * q + e] = have ? sum_grad1<RB, GT>(t.g, R, i + o) : 0.f;
         x.w[4 * q + e] = have ? t.w[i + o] : 0.f;
         cm[e] = have ? m_[im + o] : 0u, cr[e] = have ? r_[im + o] : 0u;
@@ -432,13 +425,13 @@ __device__ __forceinline__ void quant_step(QuantUnit &x, const AdamWArgs &a, flo
 __device__ __forceinline__ void put_scale(const QuantUnit &x, unsigned char *scale) {
   if ((threadIdx.x & 31) == 0) *reinterpret_cast<unsigned short *>(scale) = (unsigned short)x.scale;
 }
-template <int RB, typename GT, bool VEC, bool ALL, typename Index>
+template <int RB, typename GT, bool VEC, typename Index>
 __device__ __forceinline__ void unit_quant(const View<RB> &t, const AdamWArgs &a, int R, float s,
                                            float decay, Index i, int avail, unsigned long long place,
                                            unsigned char *m_, unsigned char *r_, Index im,
                                            unsigned char *scale) {
   QuantUnit x;
-  quant_load<RB, GT, VEC, ALL>(x, t, R, i, avail, m_, r_, im, scale);
+  quant_load<RB, GT, VEC>(x, t, R, i, avail, m_, r_, im, scale);
   quant_step<VEC>(x, a, s, decay, place, [&] {
 #pragma unroll
     for (int q = 0; q < 2; ++q) {
@@ -448,7 +441,7 @@ __device__ __forceinline__ void unit_quant(const View<RB> &t, const AdamWArgs &a
       } else {
 #pragma unroll
         for (int e = 4 * q; e < 4 * q + 4; ++e)
-          if (ALL || quant_at<false>(e) < avail) put_w1<RB>(t, R, a.lp_kind, i + (Index)quant_at<false>(e), x.w[e]);
+          if (quant_at<false>(e) < avail) put_w1<RB>(t, R, a.lp_kind, i + (Index)quant_at<false>(e), x.w[e]);
       }
     }
   });
@@ -461,7 +454,7 @@ __device__ __forceinline__ void unit_quant(const View<RB> &t, const AdamWArgs &a
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const Index o = quant_at<false>(4 * q + e);
-        if (ALL || (int)o < avail) m_[im + o] = (unsigned char)(x.m[q] >> (8 * e)), r_[im + o] = (unsigned char)(x.r[q] >> (8 * e));
+        if ((int)o < avail) m_[im + o] = (unsigned char)(x.m[q] >> (8 * e)), r_[im + o] = (unsigned char)(x.r[q] >> (8 * e));
       }
     }
   }
@@ -479,28 +472,20 @@ __device__ __forceinline__ void unit_inside(const View<RB> &t, const AdamWArgs &
     unsigned char *m = (unsigned char *)a.m, *r = (unsigned char *)a.v;
     unsigned char *scale = a.scale + e / kListUnitGroups * 2;
     if (vec && avail == kListUnit)
-      unit_quant<RB, GT, true, true>(t, a, R, s, decay, i, avail, a.flat0 + im, m, r, im, scale);
+      unit_quant<RB, GT, true>(t, a, R, s, decay, i, avail, a.flat0 + im, m, r, im, scale);
     else
-      unit_quant<RB, GT, false, false>(t, a, R, s, decay, i, avail, a.flat0 + im, m, r, im, scale);
+      unit_quant<RB, GT, false>(t, a, R, s, decay, i, avail, a.flat0 + im, m, r, im, scale);
   } else {
     float *m = (float *)a.m, *v = (float *)a.v;
     if (vec && avail == kListUnit)
       unit_vec<RB, GT>(t, a, R, s, decay, i, m, v, im);
     else
-      unit_scalar<RB, GT, 32, false>(t, a, R, s, decay, i + lane, avail > lane ? (avail - lane + 31) / 32 : 0, m, v,
+      unit_scalar<RB, GT, 32>(t, a, R, s, decay, i + lane, avail > lane ? (avail - lane + 31) / 32 : 0, m, v,
                                      im + lane);
   }
 }
 
 // ---- the kernels -----------------------------------------------------------------
-// Threads of a CTA and CTAs of an SM, fp32 moments.
-template <bool PACKED, typename GT> struct Shape {
-  static constexpr int kThreads = PACKED ? COCO_ADAMW_PACKED_THREADS
-                                  : sizeof(GT) == 4 ? COCO_ADAMW_THREADS32 : COCO_ADAMW_THREADS16;
-  static constexpr int kCtas = PACKED ? COCO_ADAMW_PACKED_CTAS
-                               : sizeof(GT) == 4 ? COCO_ADAMW_CTAS32 : COCO_ADAMW_CTAS16;
-};
-
 // A CTA's tile that holds several tensors or the end of one: every warp finds its
 // own unit.  Kept apart from the kernel's loop, whose registers decide its speed.
 template <bool QUANT, typename GT, int CAP>
@@ -527,17 +512,16 @@ __device__ __noinline__ void tile_general(const ListTable<CAP> *tab, const AdamW
     t.g[0] = tab->g[kl], t.w = tab->w[kl], t.lp = tab->lp[kl];
     const int nv = el + 1 < s_off[kl + 1] ? kListGroup : kListGroup - tab->missing[kl];
     const size_t im = (size_t)el * kListGroup;
-    unit_scalar<1, GT, 1, false>(t, a, 1, s, tab->flags[kl] & kListDecays ? a.decay : 1.f,
+    unit_scalar<1, GT, 1>(t, a, 1, s, tab->flags[kl] & kListDecays ? a.decay : 1.f,
                                  (size_t)(el - s_off[kl]) * kListGroup, nv, (float *)a.m, (float *)a.v, im);
   }
 }
 
-// A CTA takes tiles of one unit per warp.  Where a tile lies in one tensor, which and
-// where is the same for all threads: it costs no vector registers, and an element's
-// address is a common base and a 32-bit offset.  PACKED: such tiles have a form for
-// tensors that are not aligned, too.
-template <bool PACKED, typename GT, int CAP>
-__global__ void __launch_bounds__((Shape<PACKED, GT>::kThreads), (Shape<PACKED, GT>::kCtas))
+// fp32 moments, tensors that are aligned.  A CTA takes tiles of one unit per warp.
+// Where a tile lies in one tensor, which and where is the same for all threads: it costs
+// no vector registers, and an element's address is a common base and a 32-bit offset.
+template <typename GT, int CAP>
+__global__ void __launch_bounds__(COCO_ADAMW_THREADS, 2)
     adamw_kernel(const __grid_constant__ ListTable<CAP> tab, const __grid_constant__ AdamWArgs a) {
   __shared__ unsigned s_off[CAP + 1];
   const ListTable<CAP> *tp = &tab;
@@ -549,10 +533,10 @@ __global__ void __launch_bounds__((Shape<PACKED, GT>::kThreads), (Shape<PACKED, 
     s = __fmul_rn(a.norm[1], s);
   }
   __syncthreads();
-  constexpr unsigned kTile = Shape<PACKED, GT>::kThreads / 32 * kListUnitGroups;
+  constexpr unsigned kTile = COCO_ADAMW_THREADS / 32 * kListUnitGroups;
   const int n = a.n;
   const unsigned tiles = (tab.off[n] + kTile - 1) / kTile;
-  const unsigned lane = threadIdx.x & 31, mine = (threadIdx.x & ~31u) * 8;  // elements before this warp's in the tile
+  const unsigned mine = (threadIdx.x & ~31u) * 8;  // elements before this warp's in the tile
   int k = 0;  // the tensor in which the tile begins
   for (unsigned tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
     const unsigned e = tile * kTile;
@@ -560,44 +544,40 @@ __global__ void __launch_bounds__((Shape<PACKED, GT>::kThreads), (Shape<PACKED, 
     while (k + jump < n && tab.off[k + jump] <= e) k += jump, jump *= 2;
     for (; jump > 0; jump >>= 1)
       if (k + jump < n && tab.off[k + jump] <= e) k += jump;
-    const unsigned end = tab.off[k + 1];
-    const bool aligned = (tab.flags[k] & kListAligned) != 0;
     // the last group of a tensor may be short
-    if (e + kTile < end + (tab.missing[k] == 0) && (PACKED || aligned)) {
+    if (e + kTile < tab.off[k + 1] + (tab.missing[k] == 0) && (tab.flags[k] & kListAligned)) {
       const size_t i = (size_t)(e - tab.off[k]) * kListGroup, im = (size_t)e * kListGroup;
       View<1> t;
       t.g[0] = (const GT *)tab.g[k] + i;
       t.w = tab.w[k] + i;
       t.lp = (unsigned short *)tab.lp[k] + i;
-      const float decay = tab.flags[k] & kListDecays ? a.decay : 1.f;
-      float *m = (float *)a.m + im, *v = (float *)a.v + im;
-      if (!PACKED || aligned)
-        unit_vec<1, GT>(t, a, 1, s, decay, mine, m, v, mine);
-      else
-        unit_scalar<1, GT, 32, true>(t, a, 1, s, decay, mine + lane, 8, m, v, mine + lane);
+      unit_vec<1, GT>(t, a, 1, s, tab.flags[k] & kListDecays ? a.decay : 1.f, mine, (float *)a.m + im,
+                      (float *)a.v + im, mine);
     } else {
       tile_general<false, GT, CAP>(tp, a, s_off, s, tile);
     }
   }
 }
 
-// ---- 8-bit moments: tiles staged in shared memory ------------------------------------
-// The same walk with the loads in the hands of the copy engine: one thread asks for whole
-// tiles (bulk copies of the gradients, weights, codes and scales) two tiles ahead, so
+// ---- tiles staged in shared memory -----------------------------------------------------
+// The same walk with the loads in the hands of the copy engine: one warp asks for whole
+// tiles (bulk copies of the gradients, weights, moments and scales) ahead of time, so
 // that a warp finds its unit in shared memory and neither waits for HBM nor holds
-// registers for what is on its way.  A tile of a tensor that is not aligned is copied
-// from the 16-byte boundary below its start to the one above its end (memory of the same
-// allocation); its new weights leave through shared memory, in 16-byte stores but for
-// the ends of a unit.
-template <bool PACKED, typename GT> struct Pipe {
-  static constexpr int kThreads = COCO_ADAMW_QUANT_THREADS, kCtas = COCO_ADAMW_QUANT_CTAS;
+// registers for what is on its way.  8-bit moments, whose arithmetic leaves little room,
+// and tensors that are not aligned: a tile of those is copied from the 16-byte boundary
+// below its start to the one above its end (memory of the same allocation), and its new
+// weights leave through shared memory, in 16-byte stores but for the ends of a unit.
+template <bool QUANT, bool PACKED, typename GT> struct Pipe {
+  static constexpr int kThreads = QUANT ? COCO_ADAMW_QUANT_THREADS : COCO_ADAMW_PACKED_THREADS, kCtas = 2;
   static constexpr int kWarps = kThreads / 32, kTile = kWarps * kListUnit, kPad = PACKED ? 16 : 0;
+  static constexpr int kState = kTile * (QUANT ? 1 : 4);  // bytes of m and of v
   static constexpr int kG = 0, kW = kG + kTile * (int)sizeof(GT) + kPad, kM = kW + kTile * 4 + kPad;
-  static constexpr int kR = kM + kTile, kScale = kR + kTile, kBytes = kScale + (kWarps * 2 + 15) / 16 * 16 + 16;
+  static constexpr int kV = kM + kState, kScale = kV + kState;
+  static constexpr int kBytes = kScale + (QUANT ? (kWarps * 2 + 15) / 16 * 16 + 16 : 0);
   static constexpr int kLp = PACKED ? kWarps * (kListUnit * 2 + 16) : 0;  // copies on their way out
   // of an SM's 228 KB: 1 KB per CTA is reserved, 5 KB are the kernel's other tables
   static constexpr int kFit = ((228 * 1024) / kCtas - 6 * 1024 - kLp) / kBytes;
-  static constexpr int kStages = kFit < 3 ? kFit : 3;
+  static constexpr int kStages = kFit < COCO_ADAMW_STAGES ? kFit : COCO_ADAMW_STAGES;
   static_assert(kStages >= 2 && kBytes % 16 == 0, "a tile is loaded while another is worked on");
   static constexpr int kSmem = kStages * kBytes + kLp;
 };
@@ -606,22 +586,20 @@ __device__ __forceinline__ unsigned window(const void *p, unsigned n) {
   return ((unsigned)((uintptr_t)p & 15u) + n + 15u) & ~15u;
 }
 __device__ __forceinline__ const void *floor16(const void *p) { return (const void *)((uintptr_t)p & ~(uintptr_t)15u); }
-// n elements of T that lie in shared memory at the offset that p has within its 16
-// bytes, to p: whole 16-byte pieces at once, the ends one by one.
-template <typename T> __device__ __forceinline__ void store_window(T *p, const unsigned char *src, int n) {
-  constexpr int kN = 16 / (int)sizeof(T);
-  const int head = (int)((uintptr_t)p & 15u) / (int)sizeof(T);
+// A unit of T that lies in shared memory at the offset that p has within its 16 bytes,
+// to p: whole 16-byte pieces at once, what is left at the two ends one by one.
+template <typename T> __device__ __forceinline__ void store_unit(T *p, const unsigned char *src) {
+  constexpr int kN = 16 / (int)sizeof(T), kPieces = kListUnit / kN;
+  const int lane = threadIdx.x & 31, head = (int)((uintptr_t)p & 15u) / (int)sizeof(T);
   T *first = p - head;
   const T *from = reinterpret_cast<const T *>(src);
-  const int end = head + n;
-  for (int c = (threadIdx.x & 31) * kN; c < end; c += 32 * kN) {
-    if (c >= head && c + kN <= end) {
-      *reinterpret_cast<uint4 *>(first + c) = *reinterpret_cast<const uint4 *>(from + c);
-    } else {
 #pragma unroll
-      for (int j = 0; j < kN; ++j)
-        if (c + j >= head && c + j < end) first[c + j] = from[c + j];
-    }
+  for (int c = 0; c < kPieces; c += 32)
+    if (c + lane > 0 || head == 0)
+      reinterpret_cast<uint4 *>(first)[c + lane] = reinterpret_cast<const uint4 *>(from)[c + lane];
+  if (head != 0 && lane < kN) {
+    const int e = lane >= head ? lane : kListUnit + lane;
+    first[e] = from[e];
   }
 }
 
@@ -635,10 +613,10 @@ struct TileInfo {
   unsigned g_off;  // bytes between 16-byte boundaries and its gradients
 };
 
-template <bool PACKED, typename GT, int CAP>
-__global__ void __launch_bounds__((Pipe<PACKED, GT>::kThreads), (Pipe<PACKED, GT>::kCtas))
-    adamw8_kernel(const __grid_constant__ ListTable<CAP> tab, const __grid_constant__ AdamWArgs a) {
-  typedef Pipe<PACKED, GT> P;
+template <bool QUANT, bool PACKED, typename GT, int CAP>
+__global__ void __launch_bounds__((Pipe<QUANT, PACKED, GT>::kThreads), (Pipe<QUANT, PACKED, GT>::kCtas))
+    adamw_staged_kernel(const __grid_constant__ ListTable<CAP> tab, const __grid_constant__ AdamWArgs a) {
+  typedef Pipe<QUANT, PACKED, GT> P;
   constexpr unsigned S = P::kStages, kTileGroups = P::kTile / kListGroup;
   extern __shared__ __align__(128) unsigned char s_stage[];
   __shared__ unsigned s_off[CAP + 1];
@@ -668,7 +646,7 @@ __global__ void __launch_bounds__((Pipe<PACKED, GT>::kThreads), (Pipe<PACKED, GT
     if (lane == 0) {
       const bool staged = e + kTileGroups < s_off[k + 1] + (tp->missing[k] == 0) &&  // its last group may be short
                           (PACKED ? a.state_aligned != 0 : (tp->flags[k] & kListAligned) != 0);
-      const size_t i = (size_t)(e - s_off[k]) * kListGroup, im = (size_t)e * kListGroup;
+      const size_t i = (size_t)(e - s_off[k]) * kListGroup, im = (size_t)tile * P::kState;
       const GT *g = (const GT *)tp->g[k] + i;
       float *w = tp->w[k] + i;
       TileInfo &info = s_info[st];
@@ -681,13 +659,13 @@ __global__ void __launch_bounds__((Pipe<PACKED, GT>::kThreads), (Pipe<PACKED, GT
         unsigned char *dst = s_stage + st * P::kBytes;
         const unsigned char *scale = a.scale + (size_t)tile * P::kWarps * 2;
         const unsigned gb = window(g, P::kTile * (unsigned)sizeof(GT)), wb = window(w, P::kTile * 4);
-        const unsigned sb = window(scale, P::kWarps * 2);
-        mbar_expect_tx(&s_full[st], gb + wb + P::kTile * 2 + sb);
+        const unsigned sb = QUANT ? window(scale, P::kWarps * 2) : 0;
+        mbar_expect_tx(&s_full[st], gb + wb + P::kState * 2 + sb);
         bulk_load(dst + P::kG, floor16(g), gb, &s_full[st]);
         bulk_load(dst + P::kW, floor16(w), wb, &s_full[st]);
-        bulk_load(dst + P::kM, (const unsigned char *)a.m + im, P::kTile, &s_full[st]);
-        bulk_load(dst + P::kR, (const unsigned char *)a.v + im, P::kTile, &s_full[st]);
-        bulk_load(dst + P::kScale, floor16(scale), sb, &s_full[st]);
+        bulk_load(dst + P::kM, (const unsigned char *)a.m + im, P::kState, &s_full[st]);
+        bulk_load(dst + P::kV, (const unsigned char *)a.v + im, P::kState, &s_full[st]);
+        if (QUANT) bulk_load(dst + P::kScale, floor16(scale), sb, &s_full[st]);
       } else {
         mbar_arrive(&s_full[st]);
       }
@@ -728,11 +706,8 @@ __global__ void __launch_bounds__((Pipe<PACKED, GT>::kThreads), (Pipe<PACKED, GT
       const unsigned char *gs = src + P::kG + (PACKED ? info.g_off : 0) + mine * sizeof(GT);
       unsigned char *ws = src + P::kW + mine * 4;  // at a 16-byte boundary
       const unsigned w_off = PACKED ? (unsigned)((uintptr_t)w & 15u) : 0;
-      QuantUnit x;
-#pragma unroll
-      for (int q = 0; q < 2; ++q) {
+      auto take = [&](int q, float (&g4)[4], float (&w4)[4]) {
         const unsigned o = 4 * lane + 128 * q;
-        float g4[4], w4[4];
         if (aligned) {
           widen4<GT>(*reinterpret_cast<const typename Raw<GT>::Four *>(gs + o * sizeof(GT)), g4);
           widen4<float>(*reinterpret_cast<const uint4 *>(ws + o * 4), w4);
@@ -743,23 +718,19 @@ __global__ void __launch_bounds__((Pipe<PACKED, GT>::kThreads), (Pipe<PACKED, GT
             w4[j] = reinterpret_cast<const float *>(ws + w_off)[o + j];
           }
         }
-        x.m[q] = *reinterpret_cast<const unsigned *>(src + P::kM + mine + o);
-        x.r[q] = *reinterpret_cast<const unsigned *>(src + P::kR + mine + o);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) x.g[4 * q + j] = g4[j], x.w[4 * q + j] = w4[j];
-      }
-      unsigned char *scale = a.scale + ((size_t)tile * P::kWarps + wid) * 2;
-      x.scale = *reinterpret_cast<const unsigned short *>(
-          src + P::kScale + ((uintptr_t)(a.scale + (size_t)tile * P::kWarps * 2) & 15u) + wid * 2);
-      __syncwarp();
-      if (aligned && lane == 0) mbar_arrive(&s_empty[st]);
-      quant_step<true>(x, a, s, decay, a.flat0 + im + mine, [&] {
+      };
+      // this lane has taken all that it reads of the stage
+      auto taken = [&] {
+        __syncwarp();
+        if (aligned && lane == 0) mbar_arrive(&s_empty[st]);
+      };
+      auto give = [&](const float (&x)[8]) {
         if (aligned) {
           View<1> t;
           t.w = w, t.lp = lp;
 #pragma unroll
           for (int q = 0; q < 2; ++q) {
-            const float w4[4] = {x.w[4 * q], x.w[4 * q + 1], x.w[4 * q + 2], x.w[4 * q + 3]};
+            const float w4[4] = {x[4 * q], x[4 * q + 1], x[4 * q + 2], x[4 * q + 3]};
             put_w4<1>(t, 1, a.lp_kind, 4 * lane + 128 * q, w4);
           }
           return;
@@ -768,30 +739,74 @@ __global__ void __launch_bounds__((Pipe<PACKED, GT>::kThreads), (Pipe<PACKED, GT
         float *wo = reinterpret_cast<float *>(ws + w_off);
         unsigned short *lo = reinterpret_cast<unsigned short *>(ls + ((uintptr_t)lp & 15u));
 #pragma unroll
-        for (int k = 0; k < 8; ++k) {
-          const unsigned o = quant_at<true>(k);
-          wo[o] = x.w[k];
-          if (a.lp_kind == kLpF16) lo[o] = Bits16<__half>::from_f32(x.w[k]);
-          else if (a.lp_kind == kLpBf16) lo[o] = Bits16<__nv_bfloat16>::from_f32(x.w[k]);
+        for (int k = 0; k < 8; ++k) wo[quant_at<true>(k)] = x[k];
+        if (a.lp_kind != kLpNone) {
+#pragma unroll
+          for (int k = 0; k < 8; k += 2) {
+            const unsigned two = lp_pair(a.lp_kind, x[k], x[k + 1]);
+            lo[quant_at<true>(k)] = (unsigned short)two;
+            lo[quant_at<true>(k + 1)] = (unsigned short)(two >> 16);
+          }
         }
         __syncwarp();
-        store_window(w, ws, kListUnit);
-        if (a.lp_kind != kLpNone) store_window(lp, ls, kListUnit);
+        store_unit(w, ws);
+        if (a.lp_kind != kLpNone) store_unit(lp, ls);
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // before the next copy into this stage
         __syncwarp();
         if (lane == 0) mbar_arrive(&s_empty[st]);
-      });
-      unsigned char *m = (unsigned char *)a.m + im, *r = (unsigned char *)a.v + im;
+      };
+      if constexpr (QUANT) {
+        QuantUnit x;
 #pragma unroll
-      for (int q = 0; q < 2; ++q) {
-        const unsigned o = mine + 4 * lane + 128 * q;
-        *reinterpret_cast<unsigned *>(m + o) = x.m[q];
-        *reinterpret_cast<unsigned *>(r + o) = x.r[q];
+        for (int q = 0; q < 2; ++q) {
+          const unsigned o = mine + 4 * lane + 128 * q;
+          float g4[4], w4[4];
+          take(q, g4, w4);
+          x.m[q] = *reinterpret_cast<const unsigned *>(src + P::kM + o);
+          x.r[q] = *reinterpret_cast<const unsigned *>(src + P::kV + o);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) x.g[4 * q + j] = g4[j], x.w[4 * q + j] = w4[j];
+        }
+        unsigned char *scale = a.scale + ((size_t)tile * P::kWarps + wid) * 2;
+        x.scale = *reinterpret_cast<const unsigned short *>(
+            src + P::kScale + ((uintptr_t)(a.scale + (size_t)tile * P::kWarps * 2) & 15u) + wid * 2);
+        taken();
+        quant_step<true>(x, a, s, decay, a.flat0 + im + mine, [&] { give(x.w); });
+        unsigned char *m = (unsigned char *)a.m + im, *r = (unsigned char *)a.v + im;
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+          const unsigned o = mine + 4 * lane + 128 * q;
+          *reinterpret_cast<unsigned *>(m + o) = x.m[q];
+          *reinterpret_cast<unsigned *>(r + o) = x.r[q];
+        }
+        put_scale(x, scale);
+      } else {
+        float g[8], x[8], m[8], v[8];
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+          const unsigned o = mine + 4 * lane + 128 * q;
+          float g4[4], w4[4], m4[4], v4[4];
+          take(q, g4, w4);
+          widen4<float>(*reinterpret_cast<const uint4 *>(src + P::kM + o * 4), m4);
+          widen4<float>(*reinterpret_cast<const uint4 *>(src + P::kV + o * 4), v4);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) g[4 * q + j] = g4[j], x[4 * q + j] = w4[j], m[4 * q + j] = m4[j], v[4 * q + j] = v4[j];
+        }
+        taken();
+#pragma unroll
+        for (int k = 0; k < 8; ++k) update1(a, decay, __fmul_rn(g[k], s), x[k], m[k], v[k]);
+        float *mo = (float *)a.m + im, *vo = (float *)a.v + im;
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+          const unsigned o = mine + 4 * lane + 128 * q;
+          *reinterpret_cast<float4 *>(mo + o) = make_float4(m[4 * q], m[4 * q + 1], m[4 * q + 2], m[4 * q + 3]);
+          *reinterpret_cast<float4 *>(vo + o) = make_float4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
+        }
+        give(x);
       }
-      put_scale(x, scale);
     } else {
       if (lane == 0) mbar_arrive(&s_empty[st]);
-      tile_general<true, GT, CAP>(tp, a, s_off, s, tile);
+      tile_general<QUANT, GT, CAP>(tp, a, s_off, s, tile);
     }
     if (++st == S) st = 0, phase ^= 1u;
   }
@@ -841,7 +856,7 @@ __global__ void __launch_bounds__(COCO_ADAMW_PEER_THREADS, 2)
         const PeerPiece &pl = pieces[bisect(k, n - 1, el, [&](int x) { return pieces[x].off; })];
         const size_t done = (size_t)(el - pl.off) * kListGroup, left = (size_t)pl.len - done;
         const View<RB> t = {pl.g, pl.out, pl.w};
-        unit_scalar<RB, GT, 1, false>(t, a, R, s, pl.decays ? a.decay : 1.f, (size_t)pl.begin + done,
+        unit_scalar<RB, GT, 1>(t, a, R, s, pl.decays ? a.decay : 1.f, (size_t)pl.begin + done,
                                       left < kListGroup ? (int)left : kListGroup, (float *)a.m, (float *)a.v,
                                       (size_t)el * kListGroup);
       }
@@ -857,19 +872,21 @@ struct LaunchShape {
   int threads, ctas_per_sm, smem;
 };
 template <bool QUANT, bool PACKED, typename GT, int CAP> Kernel<CAP> pick_one(LaunchShape *sh) {
-  if constexpr (QUANT) {
-    typedef Pipe<PACKED, GT> P;
+  if constexpr (QUANT || PACKED) {
+    typedef Pipe<QUANT, PACKED, GT> P;
     *sh = {P::kThreads, P::kCtas, P::kSmem};
-    return adamw8_kernel<PACKED, GT, CAP>;
+    return adamw_staged_kernel<QUANT, PACKED, GT, CAP>;
   } else {
-    typedef Shape<PACKED, GT> S;
-    *sh = {S::kThreads, S::kCtas, 0};
-    return adamw_kernel<PACKED, GT, CAP>;
+    *sh = {COCO_ADAMW_THREADS, 2, 0};
+    return adamw_kernel<GT, CAP>;
   }
 }
 template <int CAP> Kernel<CAP> pick(bool quant, bool packed, cocoDataType_t g, LaunchShape *sh) {
   auto of = [&](auto type) -> Kernel<CAP> {
     typedef decltype(type) GT;
+#ifdef ALLSTAGED
+    packed = packed || !quant;
+#endif
     return quant ? packed ? pick_one<true, true, GT, CAP>(sh) : pick_one<true, false, GT, CAP>(sh)
            : packed ? pick_one<false, true, GT, CAP>(sh) : pick_one<false, false, GT, CAP>(sh);
   };
@@ -910,8 +927,8 @@ cudaError_t launch_adamw(bool quant, bool packed, cocoDataType_t g_type, const L
   const Kernel<CAP> k = pick<CAP>(quant, packed, g_type, &sh);
   if (!k) return cudaErrorInvalidValue;
   if (sh.smem > 0) {  // more than the default: allowed once per kernel and device
-    static std::atomic<unsigned long long> allowed[2][3];
-    std::atomic<unsigned long long> &mask = allowed[packed][g_type == cocoFloat32 ? 0 : g_type == cocoFloat16 ? 1 : 2];
+    static std::atomic<unsigned long long> allowed[2][2][3];
+    std::atomic<unsigned long long> &mask = allowed[quant][packed][g_type == cocoFloat32 ? 0 : g_type == cocoFloat16 ? 1 : 2];
     const unsigned long long bit = device < 64 ? 1ull << device : 0;
     if (!(mask.load(std::memory_order_acquire) & bit)) {
       const cudaError_t e = cudaFuncSetAttribute((const void *)k, cudaFuncAttributeMaxDynamicSharedMemorySize, sh.smem);
