@@ -184,9 +184,12 @@ __device__ __forceinline__ float neg_root_any(float neg_v) {
 // Multiply and xor-shift rounds; the multipliers are binary fractions of the
 // golden ratio and of the roots of 2, 3 and 5.  Any well-mixed function would do.
 constexpr unsigned kPlaceMul = 0x9E3779B1u, kHighMul = 0x3C6EF373u;
-__host__ __device__ __forceinline__ unsigned mix_bits(unsigned x) {
+__host__ __device__ __forceinline__ unsigned mix_most(unsigned x) {
   x = (x ^ (x >> 16)) * 0x6A09E667u;
-  x = (x ^ (x >> 15)) * 0xBB67AE85u;
+  return (x ^ (x >> 15)) * 0xBB67AE85u;
+}
+__host__ __device__ __forceinline__ unsigned mix_bits(unsigned x) {
+  x = mix_most(x);
   return x ^ (x >> 16);
 }
 // Two code bytes (the low 16 bits) as numbers.
@@ -218,16 +221,20 @@ __device__ __forceinline__ BlockScale block_scale(unsigned max_bits) {
   b.factor = __uint_as_float((141u - (b.big ? e - 100u : e)) << 23);
   return b;
 }
-// x times the block's factor has the code's 7 magnitude bits on top of 20 others,
-// subnormal codes included; adding 20 random bits (16 of the hash, a one that centres
-// them, zeros) and cutting 20 off rounds up with the probability of the part cut off.
-// These put the code in the top byte; the sign stays in place.
-__device__ __forceinline__ unsigned code_m(float scaled, unsigned hash) {
-  const unsigned u = __float_as_uint(scaled) + (((hash << 4) & 0xffff0u) | 8u);
-  return (u & 0x80000000u) | ((u << 4) & 0x7fffffffu);
+// x times the block's factor has the code's 7 magnitude bits in bits 20..26, subnormal
+// codes included; adding 20 random bits (16 of the hash, a one that centres them, zeros)
+// and cutting 20 off rounds up with the probability of the part cut off.  Here both are
+// 4 bits further up, so that a multiply-add leaves the code in the top byte.  The hash's
+// low half (m) and high half (r) in place, from the hash before its last x ^ (x >> 16):
+__device__ __forceinline__ void rounding(unsigned x, unsigned &for_m, unsigned &for_r) {
+  for_r = __byte_perm(x, 0x80u, 0x5324);                       // {0x80, x2, x3, 0}
+  for_m = __byte_perm(x, 0x80u, 0x5104) ^ for_r ^ 0x80u;       // {0x80, x0 ^ x2, x1 ^ x3, 0}
 }
-__device__ __forceinline__ unsigned code_r(float scaled, unsigned hash) {
-  return (__float_as_uint(scaled) + (((hash >> 12) & 0xffff0u) | 8u)) << 4;
+__device__ __forceinline__ unsigned code_r(float scaled, unsigned random) {
+  return __float_as_uint(scaled) * 16u + random;
+}
+__device__ __forceinline__ unsigned code_m(float scaled, unsigned random) {  // with its sign
+  return (code_r(scaled, random) & 0x7fffffffu) | (__float_as_uint(scaled) & 0x80000000u);
 }
 __device__ __forceinline__ unsigned top_bytes(unsigned a, unsigned b, unsigned c, unsigned d) {
   return __byte_perm(__byte_perm(a, b, 0x0073), __byte_perm(c, d, 0x0073), 0x5410);
@@ -348,7 +355,9 @@ __device__ __forceinline__ void quant_step(QuantUnit &x, const AdamWArgs &a, flo
   const float m_scale = scale_of(x.scale & 0xffu), r_scale = scale_of(x.scale >> 8);
   float m[8], r[8];  // r: -v, then -sqrt(v)
   float m_max = 0.f, v_max = 0.f;
-  unsigned low = 0xffffffffu;
+  // no v is below 2^-100 if no root was 0 and the scale is 2^-40 or more (and beta2 1/4)
+  auto has_zero = [](unsigned codes) { return ((codes & 0x7f7f7f7fu) + 0x7f7f7f7fu & 0x80808080u) != 0x80808080u; };
+  const bool maybe_low = has_zero(x.r[0]) || has_zero(x.r[1]) || (x.scale >> 8) < 87u || a.beta2 < 0.25f;
 #pragma unroll
   for (int e = 0; e < 8; e += 2) {
     const int q = e >> 2, half = e & 2 ? 16 : 0;
@@ -359,12 +368,17 @@ __device__ __forceinline__ void quant_step(QuantUnit &x, const AdamWArgs &a, flo
     const Pair pv = fma2(mul2(r0, r0), twice(a.neg_beta2), mul2(mul2(g, g), twice(a.neg_omb2)));
     unpair(pm, m[e], m[e + 1]);
     unpair(pv, r[e], r[e + 1]);
-    // distance above -0, the smallest of those that are not 0
-    low = __vimin3_u32(low, __float_as_uint(r[e]) - 0x80000001u, __float_as_uint(r[e + 1]) - 0x80000001u);
     m_max = max_abs(m_max, m[e], m[e + 1]);
     v_max = max_abs(v_max, r[e], r[e + 1]);
   }
-  if (low < 0x0d800000u || !(v_max < __uint_as_float(0x7f800000u))) {  // some v below 2^-100, inf or nan
+  bool rare = !(v_max < __uint_as_float(0x7f800000u));  // inf or nan
+  if (maybe_low) {
+    unsigned low = 0xffffffffu;  // distance above -0, the smallest of those that are not 0
+#pragma unroll
+    for (int e = 0; e < 8; ++e) low = min(low, __float_as_uint(r[e]) - 0x80000001u);
+    rare = rare || low < 0x0d800000u;
+  }
+  if (rare) {
 #pragma unroll
     for (int e = 0; e < 8; ++e) r[e] = neg_root_any(r[e]);
   } else {
@@ -407,9 +421,10 @@ __device__ __forceinline__ void quant_step(QuantUnit &x, const AdamWArgs &a, flo
       unpair(mul2(pair(r[k], r[k + 1]), twice(-rb.factor)), z[0], z[1]);
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
-        const unsigned hash = mix_bits(first + (unsigned)(quant_at<VEC>(k + j) - quant_at<VEC>(0)) * kPlaceMul);
-        cm[e + j] = code_m(y[j], hash);
-        cr[e + j] = code_r(z[j], hash);
+        unsigned for_m, for_r;
+        rounding(mix_most(first + (unsigned)(quant_at<VEC>(k + j) - quant_at<VEC>(0)) * kPlaceMul), for_m, for_r);
+        cm[e + j] = code_m(y[j], for_m);
+        cr[e + j] = code_r(z[j], for_r);
       }
     }
     unsigned mw = top_bytes(cm[0], cm[1], cm[2], cm[3]), rw = top_bytes(cr[0], cr[1], cr[2], cr[3]);
@@ -486,14 +501,13 @@ __device__ __forceinline__ void unit_inside(const View<RB> &t, const AdamWArgs &
 }
 
 // ---- the kernels -----------------------------------------------------------------
-// A CTA's tile that holds several tensors or the end of one: every warp finds its
-// own unit.  Kept apart from the kernel's loop, whose registers decide its speed.
+// A unit that holds several tensors or the end of one, by one warp.  Kept apart from the
+// kernels' loops, whose registers decide their speed.
 template <bool QUANT, typename GT, int CAP>
-__device__ __noinline__ void tile_general(const ListTable<CAP> *tab, const AdamWArgs &a, const unsigned *s_off,
-                                          float s, unsigned tile) {
+__device__ __noinline__ void unit_general(const ListTable<CAP> *tab, const AdamWArgs &a, const unsigned *s_off,
+                                          float s, unsigned unit) {
   const int n = a.n, lane = threadIdx.x & 31;
-  const unsigned total = s_off[n];
-  const unsigned e = (tile * (blockDim.x >> 5) + (threadIdx.x >> 5)) * kListUnitGroups;
+  const unsigned total = s_off[n], e = unit * kListUnitGroups;
   if (e >= total) return;
   const int k = find_tensor(s_off, n, e);
   const unsigned end = s_off[k + 1];
@@ -513,7 +527,7 @@ __device__ __noinline__ void tile_general(const ListTable<CAP> *tab, const AdamW
     const int nv = el + 1 < s_off[kl + 1] ? kListGroup : kListGroup - tab->missing[kl];
     const size_t im = (size_t)el * kListGroup;
     unit_scalar<1, GT, 1>(t, a, 1, s, tab->flags[kl] & kListDecays ? a.decay : 1.f,
-                                 (size_t)(el - s_off[kl]) * kListGroup, nv, (float *)a.m, (float *)a.v, im);
+                          (size_t)(el - s_off[kl]) * kListGroup, nv, (float *)a.m, (float *)a.v, im);
   }
 }
 
@@ -554,7 +568,7 @@ __global__ void __launch_bounds__(COCO_ADAMW_THREADS, 2)
       unit_vec<1, GT>(t, a, 1, s, tab.flags[k] & kListDecays ? a.decay : 1.f, mine, (float *)a.m + im,
                       (float *)a.v + im, mine);
     } else {
-      tile_general<false, GT, CAP>(tp, a, s_off, s, tile);
+      unit_general<false, GT, CAP>(tp, a, s_off, s, tile * (COCO_ADAMW_THREADS / 32) + (threadIdx.x >> 5));
     }
   }
 }
@@ -567,11 +581,14 @@ __global__ void __launch_bounds__(COCO_ADAMW_THREADS, 2)
 // and tensors that are not aligned: a tile of those is copied from the 16-byte boundary
 // below its start to the one above its end (memory of the same allocation), and its new
 // weights leave through shared memory, in 16-byte stores but for the ends of a unit.
+// Where a tile holds several tensors its units are copied one by one.
 template <bool QUANT, bool PACKED, typename GT> struct Pipe {
   static constexpr int kThreads = QUANT ? COCO_ADAMW_QUANT_THREADS : COCO_ADAMW_PACKED_THREADS, kCtas = 2;
-  static constexpr int kWarps = kThreads / 32, kTile = kWarps * kListUnit, kPad = PACKED ? 16 : 0;
+  static constexpr int kWarps = kThreads / 32, kTile = kWarps * kListUnit;
   static constexpr int kState = kTile * (QUANT ? 1 : 4);  // bytes of m and of v
-  static constexpr int kG = 0, kW = kG + kTile * (int)sizeof(GT) + kPad, kM = kW + kTile * 4 + kPad;
+  // the gradients and weights of a tile, or of its units one by one
+  static constexpr int kPad = PACKED ? 16 : 0, kGUnit = kListUnit * (int)sizeof(GT) + kPad, kWUnit = kListUnit * 4 + kPad;
+  static constexpr int kG = 0, kW = kG + kWarps * kGUnit, kM = kW + kWarps * kWUnit;
   static constexpr int kV = kM + kState, kScale = kV + kState;
   static constexpr int kBytes = kScale + (QUANT ? (kWarps * 2 + 15) / 16 * 16 + 16 : 0);
   static constexpr int kLp = PACKED ? kWarps * (kListUnit * 2 + 16) : 0;  // copies on their way out
@@ -603,14 +620,13 @@ template <typename T> __device__ __forceinline__ void store_unit(T *p, const uns
   }
 }
 
-// What the asker of a tile has found out about it, beside its data.
-struct TileInfo {
+// What the asker of a tile has found out about one of its units.
+struct UnitInfo {
   float *w;
   unsigned short *lp;
-  int k;           // the tensor in which it begins
-  int staged;      // its data has been asked for: it lies in one tensor
+  unsigned g_at, w_at;  // where its gradients and weights begin in the stage, in bytes
   float decay;
-  unsigned g_off;  // bytes between 16-byte boundaries and its gradients
+  int staged;           // they are asked for: the unit is whole and in one tensor
 };
 
 template <bool QUANT, bool PACKED, typename GT, int CAP>
@@ -621,7 +637,8 @@ __global__ void __launch_bounds__((Pipe<QUANT, PACKED, GT>::kThreads), (Pipe<QUA
   extern __shared__ __align__(128) unsigned char s_stage[];
   __shared__ unsigned s_off[CAP + 1];
   __shared__ __align__(8) unsigned long long s_full[S], s_empty[S];
-  __shared__ __align__(16) TileInfo s_info[S];
+  __shared__ __align__(16) UnitInfo s_info[S][P::kWarps];
+  __shared__ int s_tensor[S];  // the tensor in which a stage's tile begins
   const ListTable<CAP> *tp = &tab;
   hide(tp);
   copy_offsets(s_off, tp->off, a.n);
@@ -640,36 +657,57 @@ __global__ void __launch_bounds__((Pipe<QUANT, PACKED, GT>::kThreads), (Pipe<QUA
   const unsigned lane = threadIdx.x & 31, wid = threadIdx.x >> 5, mine = wid * kListUnit;
 
   // Asks for a tile into a free stage; by one warp, k: a tensor at or before the tile's.
+  // Lane l looks after unit l.
   auto ask = [&](unsigned tile, unsigned st, int k) {
-    const unsigned e = tile * kTileGroups;
+    const unsigned e = tile * kTileGroups, el = e + lane * kListUnitGroups, total = s_off[a.n];
     k += find_tensor(s_off + k, a.n - k, e);
-    if (lane == 0) {
-      const bool staged = e + kTileGroups < s_off[k + 1] + (tp->missing[k] == 0) &&  // its last group may be short
-                          (PACKED ? a.state_aligned != 0 : (tp->flags[k] & kListAligned) != 0);
-      const size_t i = (size_t)(e - s_off[k]) * kListGroup, im = (size_t)tile * P::kState;
-      const GT *g = (const GT *)tp->g[k] + i;
-      float *w = tp->w[k] + i;
-      TileInfo &info = s_info[st];
-      info.w = w, info.lp = (unsigned short *)tp->lp[k] + i;
-      info.k = k;
+    const bool mine_too = lane < P::kWarps && el < total;
+    int kl = k;
+    if (mine_too && el >= s_off[k + 1]) kl = bisect(k, a.n - 1, el, [&](int x) { return s_off[x]; });
+    const unsigned char flags = tab.flags[kl];  // mostly one tensor: the constant bank answers at once
+    const bool staged = mine_too && (size_t)(s_off[kl + 1] - el) * kListGroup >= (size_t)kListUnit + tab.missing[kl] &&
+                        (PACKED ? a.state_aligned != 0 : (flags & kListAligned) != 0);
+    const size_t i = mine_too ? (size_t)(el - s_off[kl]) * kListGroup : 0;
+    const GT *g = (const GT *)tab.g[kl] + i;
+    float *w = tab.w[kl] + i;
+    const unsigned g_head = PACKED ? (unsigned)((uintptr_t)g & 15u) : 0, w_head = PACKED ? (unsigned)((uintptr_t)w & 15u) : 0;
+    // all units of one tensor: they follow one another in memory, and in the stage
+    const bool run = __all_sync(0xffffffffu, lane >= P::kWarps || (staged && kl == k));
+    if (lane < P::kWarps) {
+      UnitInfo &info = s_info[st][lane];
+      info.w = w, info.lp = (unsigned short *)tab.lp[kl] + i;
+      info.g_at = P::kG + lane * (run ? kListUnit * (unsigned)sizeof(GT) : P::kGUnit) + g_head;
+      info.w_at = P::kW + lane * (run ? kListUnit * 4u : P::kWUnit) + w_head;
+      info.decay = flags & kListDecays ? a.decay : 1.f;
       info.staged = staged;
-      info.decay = tp->flags[k] & kListDecays ? a.decay : 1.f;
-      info.g_off = (unsigned)((uintptr_t)g & 15u);
-      if (staged) {
-        unsigned char *dst = s_stage + st * P::kBytes;
+    }
+    const unsigned many = run ? P::kTile : kListUnit;
+    const unsigned gb = window(g, many * (unsigned)sizeof(GT)), wb = window(w, many * 4);
+    const bool copies = run ? lane == 0 : staged;
+    const unsigned bytes = __reduce_add_sync(0xffffffffu, copies ? gb + wb : 0u);
+    unsigned char *dst = s_stage + st * P::kBytes;
+    __syncwarp();  // the units' records, before the arrival that makes them visible
+    if (lane == 0) {
+      s_tensor[st] = k;
+      if (bytes != 0) {
+        const size_t im = (size_t)tile * P::kState;
+        // of the last tile, the groups that there are
+        const unsigned groups = total - e < kTileGroups ? total - e : kTileGroups;
+        const unsigned state = groups * (P::kState / kTileGroups);
         const unsigned char *scale = a.scale + (size_t)tile * P::kWarps * 2;
-        const unsigned gb = window(g, P::kTile * (unsigned)sizeof(GT)), wb = window(w, P::kTile * 4);
-        const unsigned sb = QUANT ? window(scale, P::kWarps * 2) : 0;
-        mbar_expect_tx(&s_full[st], gb + wb + P::kState * 2 + sb);
-        bulk_load(dst + P::kG, floor16(g), gb, &s_full[st]);
-        bulk_load(dst + P::kW, floor16(w), wb, &s_full[st]);
-        bulk_load(dst + P::kM, (const unsigned char *)a.m + im, P::kState, &s_full[st]);
-        bulk_load(dst + P::kV, (const unsigned char *)a.v + im, P::kState, &s_full[st]);
+        const unsigned sb = QUANT ? window(scale, groups / kListUnitGroups * 2) : 0;
+        mbar_expect_tx(&s_full[st], bytes + state * 2 + sb);
+        bulk_load(dst + P::kM, (const unsigned char *)a.m + im, state, &s_full[st]);
+        bulk_load(dst + P::kV, (const unsigned char *)a.v + im, state, &s_full[st]);
         if (QUANT) bulk_load(dst + P::kScale, floor16(scale), sb, &s_full[st]);
-      } else {
-        mbar_arrive(&s_full[st]);
       }
     }
+    __syncwarp();
+    if (copies) {
+      bulk_load(dst + P::kG + (run ? 0 : lane * P::kGUnit), floor16(g), gb, &s_full[st]);
+      bulk_load(dst + P::kW + (run ? 0 : lane * P::kWUnit), floor16(w), wb, &s_full[st]);
+    }
+    if (lane == 0 && bytes == 0) mbar_arrive(&s_full[st]);
     __syncwarp();
   };
 
@@ -682,7 +720,7 @@ __global__ void __launch_bounds__((Pipe<QUANT, PACKED, GT>::kThreads), (Pipe<QUA
   for (unsigned tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
     ok = __all_sync(0xffffffffu, mbar_wait(&s_full[st], phase, a.timeout_ns));
     if (!ok) break;
-    const TileInfo &info = s_info[st];
+    const UnitInfo &info = s_info[st][wid];
     // the warps take turns at asking for the tile S - 1 ahead, into the stage that the
     // tile before this one has left
     if (turn == wid) {
@@ -692,20 +730,19 @@ __global__ void __launch_bounds__((Pipe<QUANT, PACKED, GT>::kThreads), (Pipe<QUA
         if (tile != blockIdx.x)
           ok = __all_sync(0xffffffffu, mbar_wait(&s_empty[to], st == 0 ? phase ^ 1u : phase, a.timeout_ns));
         if (!ok) break;
-        ask(ahead, to, info.k);
+        ask(ahead, to, s_tensor[st]);
       }
     }
     turn = turn + 1 == P::kWarps ? 0 : turn + 1;
     if (info.staged) {
       unsigned char *src = s_stage + st * P::kBytes;
       const size_t im = (size_t)tile * P::kTile;
-      float *w = info.w + mine;
-      unsigned short *lp = info.lp + mine;
+      float *w = info.w;
+      unsigned short *lp = info.lp;
       const float decay = info.decay;
-      const bool aligned = !PACKED || ((info.g_off | ((uintptr_t)w & 15u) | ((uintptr_t)lp & 15u)) == 0);
-      const unsigned char *gs = src + P::kG + (PACKED ? info.g_off : 0) + mine * sizeof(GT);
-      unsigned char *ws = src + P::kW + mine * 4;  // at a 16-byte boundary
-      const unsigned w_off = PACKED ? (unsigned)((uintptr_t)w & 15u) : 0;
+      const unsigned char *gs = src + info.g_at;
+      unsigned char *ws = src + info.w_at;
+      const bool aligned = !PACKED || (((info.g_at | info.w_at) & 15u) | ((uintptr_t)lp & 15u)) == 0;
       auto take = [&](int q, float (&g4)[4], float (&w4)[4]) {
         const unsigned o = 4 * lane + 128 * q;
         if (aligned) {
@@ -715,7 +752,7 @@ __global__ void __launch_bounds__((Pipe<QUANT, PACKED, GT>::kThreads), (Pipe<QUA
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
             g4[j] = Raw<GT>::widen1(reinterpret_cast<const typename Raw<GT>::One *>(gs)[o + j]);
-            w4[j] = reinterpret_cast<const float *>(ws + w_off)[o + j];
+            w4[j] = reinterpret_cast<const float *>(ws)[o + j];
           }
         }
       };
@@ -736,7 +773,7 @@ __global__ void __launch_bounds__((Pipe<QUANT, PACKED, GT>::kThreads), (Pipe<QUA
           return;
         }
         unsigned char *ls = s_stage + S * P::kBytes + wid * (kListUnit * 2 + 16);
-        float *wo = reinterpret_cast<float *>(ws + w_off);
+        float *wo = reinterpret_cast<float *>(ws);
         unsigned short *lo = reinterpret_cast<unsigned short *>(ls + ((uintptr_t)lp & 15u));
 #pragma unroll
         for (int k = 0; k < 8; ++k) wo[quant_at<true>(k)] = x[k];
@@ -749,7 +786,7 @@ __global__ void __launch_bounds__((Pipe<QUANT, PACKED, GT>::kThreads), (Pipe<QUA
           }
         }
         __syncwarp();
-        store_unit(w, ws);
+        store_unit(w, ws - ((uintptr_t)w & 15u));
         if (a.lp_kind != kLpNone) store_unit(lp, ls);
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // before the next copy into this stage
         __syncwarp();
@@ -806,7 +843,7 @@ __global__ void __launch_bounds__((Pipe<QUANT, PACKED, GT>::kThreads), (Pipe<QUA
       }
     } else {
       if (lane == 0) mbar_arrive(&s_empty[st]);
-      tile_general<QUANT, GT, CAP>(tp, a, s_off, s, tile);
+      unit_general<QUANT, GT, CAP>(tp, a, s_off, s, tile * P::kWarps + wid);
     }
     if (++st == S) st = 0, phase ^= 1u;
   }
