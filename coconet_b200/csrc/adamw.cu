@@ -626,7 +626,7 @@ struct UnitInfo {
   unsigned short *lp;
   unsigned g_at, w_at;  // where its gradients and weights begin in the stage, in bytes
   float decay;
-  int staged;           // they are asked for: the unit is whole and in one tensor
+  int staged;           // elements that are asked for; 0: the unit is not staged
 };
 
 template <bool QUANT, bool PACKED, typename GT, int CAP>
@@ -665,14 +665,18 @@ __global__ void __launch_bounds__((Pipe<QUANT, PACKED, GT>::kThreads), (Pipe<QUA
     int kl = k;
     if (mine_too && el >= s_off[k + 1]) kl = bisect(k, a.n - 1, el, [&](int x) { return s_off[x]; });
     const unsigned char flags = tab.flags[kl];  // mostly one tensor: the constant bank answers at once
-    const bool staged = mine_too && (size_t)(s_off[kl + 1] - el) * kListGroup >= (size_t)kListUnit + tab.missing[kl] &&
-                        (PACKED ? a.state_aligned != 0 : (flags & kListAligned) != 0);
+    unsigned staged = 0;
+    if (mine_too && (PACKED ? a.state_aligned != 0 : (flags & kListAligned) != 0)) {
+      const size_t left = (size_t)(s_off[kl + 1] - el) * kListGroup - tab.missing[kl];
+      // fp32 moments: a unit that a tensor ends in may hold others
+      staged = left >= kListUnit ? kListUnit : QUANT ? (unsigned)left : 0;
+    }
     const size_t i = mine_too ? (size_t)(el - s_off[kl]) * kListGroup : 0;
     const GT *g = (const GT *)tab.g[kl] + i;
     float *w = tab.w[kl] + i;
     const unsigned g_head = PACKED ? (unsigned)((uintptr_t)g & 15u) : 0, w_head = PACKED ? (unsigned)((uintptr_t)w & 15u) : 0;
     // all units of one tensor: they follow one another in memory, and in the stage
-    const bool run = __all_sync(0xffffffffu, lane >= P::kWarps || (staged && kl == k));
+    const bool run = __all_sync(0xffffffffu, lane >= P::kWarps || (staged == kListUnit && kl == k));
     if (lane < P::kWarps) {
       UnitInfo &info = s_info[st][lane];
       info.w = w, info.lp = (unsigned short *)tab.lp[kl] + i;
@@ -681,9 +685,9 @@ __global__ void __launch_bounds__((Pipe<QUANT, PACKED, GT>::kThreads), (Pipe<QUA
       info.decay = flags & kListDecays ? a.decay : 1.f;
       info.staged = staged;
     }
-    const unsigned many = run ? P::kTile : kListUnit;
+    const unsigned many = run ? P::kTile : staged;
     const unsigned gb = window(g, many * (unsigned)sizeof(GT)), wb = window(w, many * 4);
-    const bool copies = run ? lane == 0 : staged;
+    const bool copies = run ? lane == 0 : staged != 0;
     const unsigned bytes = __reduce_add_sync(0xffffffffu, copies ? gb + wb : 0u);
     unsigned char *dst = s_stage + st * P::kBytes;
     __syncwarp();  // the units' records, before the arrival that makes them visible
@@ -742,6 +746,8 @@ __global__ void __launch_bounds__((Pipe<QUANT, PACKED, GT>::kThreads), (Pipe<QUA
       const float decay = info.decay;
       const unsigned char *gs = src + info.g_at;
       unsigned char *ws = src + info.w_at;
+      const int avail = QUANT ? info.staged : kListUnit;
+      const bool whole = !QUANT || avail == kListUnit;
       const bool aligned = !PACKED || (((info.g_at | info.w_at) & 15u) | ((uintptr_t)lp & 15u)) == 0;
       auto take = [&](int q, float (&g4)[4], float (&w4)[4]) {
         const unsigned o = 4 * lane + 128 * q;
@@ -759,12 +765,18 @@ __global__ void __launch_bounds__((Pipe<QUANT, PACKED, GT>::kThreads), (Pipe<QUA
       // this lane has taken all that it reads of the stage
       auto taken = [&] {
         __syncwarp();
-        if (aligned && lane == 0) mbar_arrive(&s_empty[st]);
+        if ((aligned || !whole) && lane == 0) mbar_arrive(&s_empty[st]);
       };
       auto give = [&](const float (&x)[8]) {
+        View<1> t;
+        t.w = w, t.lp = lp;
+        if (!whole) {
+#pragma unroll
+          for (int k = 0; k < 8; ++k)
+            if (quant_at<true>(k) < avail) put_w1<1>(t, 1, a.lp_kind, (unsigned)quant_at<true>(k), x[k]);
+          return;
+        }
         if (aligned) {
-          View<1> t;
-          t.w = w, t.lp = lp;
 #pragma unroll
           for (int q = 0; q < 2; ++q) {
             const float w4[4] = {x[4 * q], x[4 * q + 1], x[4 * q + 2], x[4 * q + 3]};
@@ -804,6 +816,14 @@ __global__ void __launch_bounds__((Pipe<QUANT, PACKED, GT>::kThreads), (Pipe<QUA
 #pragma unroll
           for (int j = 0; j < 4; ++j) x.g[4 * q + j] = g4[j], x.w[4 * q + j] = w4[j];
         }
+        if (!whole) {  // what lies behind the tensor's end is no part of it
+#pragma unroll
+          for (int k = 0; k < 8; ++k)
+            if (quant_at<true>(k) >= avail) {
+              x.g[k] = 0.f, x.w[k] = 0.f;
+              x.m[k >> 2] &= ~(0xffu << (8 * (k & 3))), x.r[k >> 2] &= ~(0xffu << (8 * (k & 3)));
+            }
+        }
         unsigned char *scale = a.scale + ((size_t)tile * P::kWarps + wid) * 2;
         x.scale = *reinterpret_cast<const unsigned short *>(
             src + P::kScale + ((uintptr_t)(a.scale + (size_t)tile * P::kWarps * 2) & 15u) + wid * 2);
@@ -813,8 +833,13 @@ __global__ void __launch_bounds__((Pipe<QUANT, PACKED, GT>::kThreads), (Pipe<QUA
 #pragma unroll
         for (int q = 0; q < 2; ++q) {
           const unsigned o = mine + 4 * lane + 128 * q;
-          *reinterpret_cast<unsigned *>(m + o) = x.m[q];
-          *reinterpret_cast<unsigned *>(r + o) = x.r[q];
+          if (whole || quant_at<true>(4 * q + 3) < avail) {
+            *reinterpret_cast<unsigned *>(m + o) = x.m[q];
+            *reinterpret_cast<unsigned *>(r + o) = x.r[q];
+          } else {
+            for (int j = 0; quant_at<true>(4 * q) + j < avail; ++j)
+              m[o + j] = (unsigned char)(x.m[q] >> (8 * j)), r[o + j] = (unsigned char)(x.r[q] >> (8 * j));
+          }
         }
         put_scale(x, scale);
       } else {
