@@ -154,13 +154,16 @@ __global__ void __launch_bounds__(COCO_NORM_THREADS, COCO_NORM_CTAS)
       for (int k = 0; k < kDepth; ++k) q[k] = p[e - begin + lane + 32 * k];
       if (head && e == begin && lane == 0) q[0] = masked<GT>(q[0], head, 0);
       if (tail && e + kUnit == end && lane == 31) q[kDepth - 1] = masked<GT>(q[kDepth - 1], 0, tail);
-    } else {  // several tensors: every group looks up its own
+    } else {  // several tensors: every group looks up its own, between the warp's first and last
+      int t_at[kDepth + 1];
+#pragma unroll
+      for (int k = 0; k <= kDepth; ++k) t_at[k] = find_tensor(s_off, n, min(e + 32 * k, total - 1));
 #pragma unroll
       for (int k = 0; k < kDepth; ++k) {
         const unsigned x = e + lane + 32 * k;
         q[k] = make_uint4(0u, 0u, 0u, 0u);
         if (x < total) {
-          const int t = bisect(0, n - 1, x, [&](int y) { return s_off[y]; });
+          const int t = bisect(t_at[k], t_at[k + 1], x, [&](int y) { return s_off[y]; });
           q[k] = ((const uint4 *)tp->g[t])[x - s_off[t]];
           const int h = x == s_off[t] ? tp->head[t] : 0, l = x == s_off[t + 1] - 1 ? tp->tail[t] : 0;
           if (h | l) q[k] = masked<GT>(q[k], h, l);
