@@ -97,21 +97,18 @@ _SIGNATURES = {
                                          C.c_void_p, C.c_float, C.c_float, C.c_float, C.c_float,
                                          C.c_float, C.c_int, C.c_float, C.c_int, C.c_uint,
                                          C.c_void_p]),
-    "cocoGradNormScattered": (C.c_int, [C.c_void_p, C.c_size_t, C.POINTER(C.c_void_p), C.c_int,
-                                        C.POINTER(C.c_size_t), C.c_float, C.c_float, C.c_void_p,
-                                        C.c_void_p]),
-    "cocoFusedAdamWScattered": (C.c_int, [C.c_void_p, C.c_size_t, C.POINTER(C.c_void_p), C.c_int,
-                                          C.POINTER(C.c_void_p), C.POINTER(C.c_void_p), C.c_int,
-                                          C.POINTER(C.c_size_t), C.c_void_p, C.c_void_p, C.c_float,
-                                          C.c_float, C.c_float, C.c_float, C.c_float,
-                                          C.POINTER(C.c_ubyte), C.c_int, C.c_float, C.c_void_p,
-                                          C.c_void_p]),
-    "cocoFusedAdamWQuantScattered": (C.c_int, [C.c_void_p, C.c_size_t, C.POINTER(C.c_void_p), C.c_int,
-                                               C.POINTER(C.c_void_p), C.POINTER(C.c_void_p), C.c_int,
-                                               C.POINTER(C.c_size_t), C.c_void_p, C.c_void_p,
+    # (arrays as plain addresses: the quickest to convert)
+    "cocoGradNormScattered": (C.c_int, [C.c_void_p, C.c_size_t, C.c_void_p, C.c_int, C.c_void_p,
+                                        C.c_float, C.c_float, C.c_void_p, C.c_void_p]),
+    "cocoFusedAdamWScattered": (C.c_int, [C.c_void_p, C.c_size_t, C.c_void_p, C.c_int, C.c_void_p,
+                                          C.c_void_p, C.c_int, C.c_void_p, C.c_void_p, C.c_void_p,
+                                          C.c_float, C.c_float, C.c_float, C.c_float, C.c_float,
+                                          C.c_void_p, C.c_int, C.c_float, C.c_void_p, C.c_void_p]),
+    "cocoFusedAdamWQuantScattered": (C.c_int, [C.c_void_p, C.c_size_t, C.c_void_p, C.c_int, C.c_void_p,
+                                               C.c_void_p, C.c_int, C.c_void_p, C.c_void_p, C.c_void_p,
                                                C.c_void_p, C.c_float, C.c_float, C.c_float, C.c_float,
-                                               C.c_float, C.POINTER(C.c_ubyte), C.c_int, C.c_uint64,
-                                               C.c_float, C.c_void_p, C.c_void_p]),
+                                               C.c_float, C.c_void_p, C.c_int, C.c_uint64, C.c_float,
+                                               C.c_void_p, C.c_void_p]),
     "cocoQuantSliceElems": (C.c_int, [C.c_size_t, C.POINTER(C.c_size_t), C.c_int,
                                       C.POINTER(C.c_size_t)]),
     "cocoQuantTensorPlace": (C.c_int, [C.c_size_t, C.POINTER(C.c_size_t), C.c_int, C.c_size_t,
@@ -329,6 +326,9 @@ class TensorList:
         self.lp = (C.c_void_p * self.n)(*[t.data_ptr() for t in lps]) if lps is not None else None
         self.lp_dtype = _dtype_code(lps[0]) if lps is not None else _F16
         self.no_decay = (C.c_ubyte * self.n)(*[1 if x else 0 for x in no_decay]) if no_decay is not None else None
+        # addresses of the arrays (gradients, weights, copies, counts, no_decay)
+        self._at = tuple(C.addressof(x) if x is not None else None
+                         for x in (self.g, self.w, self.lp, self.counts, self.no_decay))
         self._device = None   # set once the list has passed _checked
         self._slices = {}
 
@@ -565,9 +565,9 @@ class Communicator:
         lst = gs if isinstance(gs, TensorList) else TensorList(gs, None)
         device = lst._checked(weights=False)
         p = self._held(norm, "norm", device, (torch.float32,), 2)
-        _check(lib().cocoGradNormScattered(self._h, lst.n, lst.g, lst.dtype, lst.counts, grad_scale,
-                                           max_norm, p, self._on(device, stream)),
-               "cocoGradNormScattered")
+        g, _, _, counts, _ = lst._at
+        _check(lib().cocoGradNormScattered(self._h, lst.n, g, lst.dtype, counts, grad_scale, max_norm, p,
+                                           self._on(device, stream)), "cocoGradNormScattered")
 
     def fused_adamw_scattered(self, gs, ws, m, v, lr, beta1, beta2, eps, weight_decay, step,
                               w_lps=None, no_decay=None, grad_scale=1.0, norm=None, stream=None):
@@ -578,10 +578,11 @@ class Communicator:
         lst = gs if isinstance(gs, TensorList) else TensorList(gs, ws, w_lps, no_decay)
         device = lst._checked(weights=True)
         need, f32 = lst._slice(self.world, False), (torch.float32,)
+        g, w, lp, counts, no_decay = lst._at
         _check(lib().cocoFusedAdamWScattered(
-            self._h, lst.n, lst.g, lst.dtype, lst.w, lst.lp, lst.lp_dtype, lst.counts,
+            self._h, lst.n, g, lst.dtype, w, lp, lst.lp_dtype, counts,
             self._held(m, "m", device, f32, need), self._held(v, "v", device, f32, need),
-            lr, beta1, beta2, eps, weight_decay, lst.no_decay, step, grad_scale,
+            lr, beta1, beta2, eps, weight_decay, no_decay, step, grad_scale,
             self._held(norm, "norm", device, f32, 2) if norm is not None else None,
             self._on(device, stream)), "cocoFusedAdamWScattered")
 
@@ -595,11 +596,12 @@ class Communicator:
         device = lst._checked(weights=True)
         need = lst._slice(self.world, True)
         code, exponent = (torch.float8_e4m3fn, torch.uint8), (torch.float8_e8m0fnu, torch.uint8)
+        g, w, lp, counts, no_decay = lst._at
         _check(lib().cocoFusedAdamWQuantScattered(
-            self._h, lst.n, lst.g, lst.dtype, lst.w, lst.lp, lst.lp_dtype, lst.counts,
+            self._h, lst.n, g, lst.dtype, w, lp, lst.lp_dtype, counts,
             self._held(m, "m", device, code, need), self._held(vroot, "vroot", device, code, need),
             self._held(scale, "scale", device, exponent, need // QUANT_BLOCK * 2),
-            lr, beta1, beta2, eps, weight_decay, lst.no_decay, step, seed, grad_scale,
+            lr, beta1, beta2, eps, weight_decay, no_decay, step, seed, grad_scale,
             self._held(norm, "norm", device, (torch.float32,), 2) if norm is not None else None,
             self._on(device, stream)), "cocoFusedAdamWQuantScattered")
 

@@ -559,6 +559,78 @@ def test_two_graphs_of_one_communicator_replay_in_any_order(comm):
         assert torch.equal(outs[0], expect[0]) and torch.equal(outs[1], expect[1])
 
 
+@pytest.mark.parametrize("op", ["norm", "adamw", "quant"])
+def test_the_first_call_of_a_process_may_be_captured(op):
+    """A list of two launches, captured before anything of the library has run; the replay against a plain call."""
+    code = f"""
+import torch, coconet_b200 as coco
+comm = coco.Communicator.init_all(1, [0])[0]
+counts = [1 + (k * 37) % 500 for k in range(1100)]
+g = [torch.randn(c, device='cuda').bfloat16() for c in counts]
+w = [torch.randn(c, device='cuda') for c in counts]
+op = {op!r}
+def state():
+    if op == 'norm':
+        return (torch.zeros(2, device='cuda'),)
+    if op == 'quant':
+        return coco.quant_state(counts, 1)
+    return tuple(torch.zeros(coco.scattered_slice_elems(counts, 1), device='cuda') for _ in range(2))
+def call(lst, st):
+    if op == 'norm':
+        comm.grad_norm_scattered(lst, *st)
+    elif op == 'quant':
+        comm.fused_adamw_quant_scattered(lst, None, *st, 1e-3, 0.9, 0.99, 1e-8, 0.1, 2, 3)
+    else:
+        comm.fused_adamw_scattered(lst, None, *st, 1e-3, 0.9, 0.99, 1e-8, 0.1, 2)
+ws = [[x.clone() for x in w] for _ in range(2)]
+sts = [state() for _ in range(2)]
+lists = [coco.TensorList(g, x) for x in ws]
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    call(lists[0], sts[0])
+assert all(torch.equal(a, b) for a, b in zip(ws[0], w))
+graph.replay()
+call(lists[1], sts[1])
+torch.cuda.synchronize()
+assert all(torch.equal(a, b) for a, b in zip(*ws))
+assert all(torch.equal(a.view(torch.uint8), b.view(torch.uint8)) for a, b in zip(*sts))
+assert op != 'norm' or float(sts[0][0][0]) > 0
+assert op == 'norm' or not torch.equal(ws[0][1], w[1])
+assert comm.launch_count() == 4 and comm.status()['code'] == 0
+"""
+    import os
+    import subprocess
+    import sys
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    r = subprocess.run([sys.executable, "-c", code], cwd=root, capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0, r.stderr[-2000:]
+
+
+def test_calls_on_two_streams_do_not_disturb_each_other(comm):
+    """AdamW calls at world size 1 share nothing: two lists stepped on two streams at once, ten times."""
+    counts = [400003, 5, 70000]
+    w, m, v, (g,) = _make(counts, 70, "f32")
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    sets = []
+    for _ in range(3):
+        sets.append((coco.TensorList(_aligned(g, torch.float32), _aligned(w, torch.float32)),
+                     [torch.from_numpy(_flat(x, counts, 8)).cuda() for x in (m, v)],
+                     coco.TensorList(_aligned(g, torch.float32), _aligned(w, torch.float32)), coco.quant_state(counts, 1)))
+    torch.cuda.synchronize()
+    for k in range(10):
+        for lst, st, qlst, qst in sets[:1]:
+            comm.fused_adamw_scattered(lst, None, *st, H["lr"], H["beta1"], H["beta2"], H["eps"], 0.1, k)
+            comm.fused_adamw_quant_scattered(qlst, None, *qst, H["lr"], H["beta1"], H["beta2"], H["eps"], 0.1, k, 1)
+        for stream, (lst, st, qlst, qst) in zip(streams, sets[1:]):
+            comm.fused_adamw_scattered(lst, None, *st, H["lr"], H["beta1"], H["beta2"], H["eps"], 0.1, k, stream=stream)
+            comm.fused_adamw_quant_scattered(qlst, None, *qst, H["lr"], H["beta1"], H["beta2"], H["eps"], 0.1, k, 1, stream=stream)
+    torch.cuda.synchronize()
+    flat = [list(s[0].tensors[1]) + list(s[1]) + list(s[2].tensors[1]) + [x.view(torch.uint8) for x in s[3]] for s in sets]
+    for other in flat[1:]:
+        assert all(torch.equal(a, b) for a, b in zip(flat[0], other))
+
+
 def test_another_stream_and_a_group_of_one(comm):
     counts = RAGGED
     w, m, v, (g,) = _make(counts, 60, "f32")
