@@ -136,9 +136,7 @@ __device__ __forceinline__ void update1(const AdamWArgs &a, float decay, float g
 }
 
 // With 8-bit moments the instructions, not the bytes, bound the kernel: two
-// elements per instruction (f32x2), sums of products as multiply-adds.  (The
-// compiler fuses a packed multiply into a packed add whatever their rounding
-// modifiers say, so the fused form is what is written.)
+// elements per instruction (f32x2).
 typedef unsigned long long Pair;
 __device__ __forceinline__ Pair pair(float a, float b) {
   Pair p;
@@ -159,6 +157,15 @@ __device__ __forceinline__ Pair fma2(Pair a, Pair b, Pair c) {
   return p;
 }
 __device__ __forceinline__ Pair twice(float a) { return pair(a, a); }
+// a + b of products that are to be rounded first.  One by one: the compiler fuses a
+// packed multiply into a packed add whatever their rounding modifiers say, and a last
+// bit of a moment is a whole step of its code now and then.
+__device__ __forceinline__ void sum2(Pair a, Pair b, float &x, float &y) {
+  float a0, a1, b0, b1;
+  unpair(a, a0, a1);
+  unpair(b, b0, b1);
+  x = __fadd_rn(a0, b0), y = __fadd_rn(a1, b1);
+}
 // Of -v, the negative of the root as the state keeps it, rounded to nearest: with y
 // the hardware's reciprocal root of v, one Newton step r + (v - r^2) y / 2 from
 // r = v y.  The multiply-add leaves the residual exact for v from 2^-100 on; 0 gives 0.
@@ -364,10 +371,8 @@ __device__ __forceinline__ void quant_step(QuantUnit &x, const AdamWArgs &a, flo
     Pair pm = mul2(decode2(x.m[q] >> half), twice(m_scale));
     const Pair r0 = mul2(decode2(x.r[q] >> half), twice(r_scale));
     const Pair g = mul2(pair(x.g[e], x.g[e + 1]), twice(s));
-    pm = fma2(pm, twice(a.beta1), mul2(g, twice(a.omb1)));
-    const Pair pv = fma2(mul2(r0, r0), twice(a.neg_beta2), mul2(mul2(g, g), twice(a.neg_omb2)));
-    unpair(pm, m[e], m[e + 1]);
-    unpair(pv, r[e], r[e + 1]);
+    sum2(mul2(pm, twice(a.beta1)), mul2(g, twice(a.omb1)), m[e], m[e + 1]);
+    sum2(mul2(mul2(r0, r0), twice(a.neg_beta2)), mul2(mul2(g, g), twice(a.neg_omb2)), r[e], r[e + 1]);
     m_max = max_abs(m_max, m[e], m[e + 1]);
     v_max = max_abs(v_max, r[e], r[e + 1]);
   }

@@ -377,8 +377,7 @@ int cocoFusedLAMBScattered(cocoComm_t comm, size_t nbuff, const void *const *g,
  * the probability of the part cut off (to nearest, a beta2 of 0.999 would never
  * move vroot); the random bits are a function of `seed`, `step` and the element's
  * place in the flat state, so that a step is reproducible, and the same at every
- * world size.  (m and v are formed with one multiply-add each, not rounded between
- * the product and the sum.)  A vroot above 0 is never stored as 0; a block in which a moment is
+ * world size.  A vroot above 0 is never stored as 0; a block in which a moment is
  * inf or nan gets scale byte 255, which reads back as nan. */
 int cocoGradNormScattered(cocoComm_t comm, size_t nbuff, const void *const *g,
                           cocoDataType_t g_type, const size_t *counts, float grad_scale,

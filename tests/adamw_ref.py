@@ -76,23 +76,6 @@ def moments32(h, m, v, g):
     return m * h["b1"] + g * h["omb1"], v * h["b2"] + (g * g) * h["omb2"]
 
 
-def fma32(a, b, c):
-    """a * b + c rounded once.  The product of two fp32 numbers is exact in fp64; the fp64 sum is rounded to odd
-    (its last bit set when anything was cut off), which makes the second rounding, to fp32, the only one that counts."""
-    p, c = a.astype(np.float64) * float(b), c.astype(np.float64)
-    s = p + c
-    t = s - p
-    cut = (p - (s - t)) + (c - t)
-    even = (s.view(np.uint64) & np.uint64(1)) == 0
-    fix = np.isfinite(s) & (cut != 0) & even
-    return np.where(fix, np.nextafter(s, np.where(cut > 0, np.inf, -np.inf)), s).astype(F)
-
-
-def fused_moments32(h, m, v, g):
-    """The 8-bit form's: the first product goes unrounded into the sum."""
-    return fma32(m, h["b1"], g * h["omb1"]), fma32(v, h["b2"], (g * g) * h["omb2"])
-
-
 def weights32(h, w, m, r, decays):
     return w * (h["decay"] if decays else F(1)) - (m * h["c1"]) / (r * h["rs2"] + h["eps"])
 
@@ -188,7 +171,7 @@ def quant_step32(w, m_codes, r_codes, scales, g, step, seed, place, decays=True,
         sc = scale_values(scales).astype(F).repeat(BLOCK, 0)[:w.size]
         m = code_values(m_codes).astype(F) * sc[:, 0]
         r = code_values(r_codes).astype(F) * sc[:, 1]
-        m, v = fused_moments32(h, m, r * r, g)
+        m, v = moments32(h, m, r * r, g)
         r = np.sqrt(v)
         w = weights32(h, w, m, r, decays)
         bits = rounding_bits(place, w.size, seed, step)
