@@ -228,6 +228,11 @@ __device__ __forceinline__ BlockScale block_scale(unsigned max_bits) {
   b.factor = __uint_as_float((141u - (b.big ? e - 100u : e)) << 23);
   return b;
 }
+// The same where the largest magnitude lies in [2^-119, 2^14).
+__device__ __forceinline__ bool is_usual(unsigned max_bits) { return max_bits - 0x04000000u < 0x46800000u - 0x04000000u; }
+__device__ __forceinline__ BlockScale usual_scale(unsigned max_bits) {
+  return {(max_bits >> 23) - 7u, false, __uint_as_float(0x46800000u - (max_bits & 0x7f800000u))};
+}
 // x times the block's factor has the code's 7 magnitude bits in bits 20..26, subnormal
 // codes included; adding 20 random bits (16 of the hash, a one that centres them, zeros)
 // and cutting 20 off rounds up with the probability of the part cut off.  Here both are
@@ -359,16 +364,14 @@ __device__ __forceinline__ void quant_load(QuantUnit &x, const View<RB> &t, int 
 template <bool VEC, typename PutW>
 __device__ __forceinline__ void quant_step(QuantUnit &x, const AdamWArgs &a, float s, float decay,
                                            unsigned long long place, PutW put_w) {
-  const float m_scale = scale_of(x.scale & 0xffu), r_scale = scale_of(x.scale >> 8);
+  const unsigned r_byte = x.scale >> 8;
+  const float m_scale = scale_of(x.scale & 0xffu), r_scale = scale_of(r_byte);
   float m[8], r[8];  // r: -v, then -sqrt(v)
   float m_max = 0.f, v_max = 0.f;
-  // no v is below 2^-100 if no root was 0 and the scale is 2^-40 or more (and beta2 1/4)
-  auto has_zero = [](unsigned codes) { return ((codes & 0x7f7f7f7fu) + 0x7f7f7f7fu & 0x80808080u) != 0x80808080u; };
-  const bool maybe_low = has_zero(x.r[0]) || has_zero(x.r[1]) || (x.scale >> 8) < 87u || a.beta2 < 0.25f;
 #pragma unroll
   for (int e = 0; e < 8; e += 2) {
     const int q = e >> 2, half = e & 2 ? 16 : 0;
-    Pair pm = mul2(decode2(x.m[q] >> half), twice(m_scale));
+    const Pair pm = mul2(decode2(x.m[q] >> half), twice(m_scale));
     const Pair r0 = mul2(decode2(x.r[q] >> half), twice(r_scale));
     const Pair g = mul2(pair(x.g[e], x.g[e + 1]), twice(s));
     sum2(mul2(pm, twice(a.beta1)), mul2(g, twice(a.omb1)), m[e], m[e + 1]);
@@ -377,7 +380,9 @@ __device__ __forceinline__ void quant_step(QuantUnit &x, const AdamWArgs &a, flo
     v_max = max_abs(v_max, r[e], r[e + 1]);
   }
   bool rare = !(v_max < __uint_as_float(0x7f800000u));  // inf or nan
-  if (maybe_low) {
+  // no v is below 2^-100 if no root was 0 and the scale is 2^-40 or more (and beta2 1/4)
+  auto has_zero = [](unsigned codes) { return ((codes & 0x7f7f7f7fu) + 0x7f7f7f7fu & 0x80808080u) != 0x80808080u; };
+  if (has_zero(x.r[0]) || has_zero(x.r[1]) || r_byte < 87u || a.beta2 < 0.25f) {
     unsigned low = 0xffffffffu;  // distance above -0, the smallest of those that are not 0
 #pragma unroll
     for (int e = 0; e < 8; ++e) low = min(low, __float_as_uint(r[e]) - 0x80000001u);
@@ -401,17 +406,22 @@ __device__ __forceinline__ void quant_step(QuantUnit &x, const AdamWArgs &a, flo
     r_max = max_abs(r_max, r[e], r[e + 1]);
   }
   put_w();
-  const BlockScale mb = block_scale(__reduce_max_sync(0xffffffffu, __float_as_uint(m_max) & 0x7fffffffu));
-  const BlockScale rb = block_scale(__reduce_max_sync(0xffffffffu, __float_as_uint(r_max) & 0x7fffffffu));
+  const unsigned m_top = __reduce_max_sync(0xffffffffu, __float_as_uint(m_max) & 0x7fffffffu);
+  const unsigned r_top = __reduce_max_sync(0xffffffffu, __float_as_uint(r_max) & 0x7fffffffu);
+  BlockScale mb = usual_scale(m_top), rb = usual_scale(r_top);
+  const bool unusual = !is_usual(m_top) || !is_usual(r_top);
+  if (unusual) {
+    mb = block_scale(m_top), rb = block_scale(r_top);
+    if (mb.big) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) m[e] *= 0x1p-100f;
+    }
+    if (rb.big) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) r[e] = r[e] < 0.f ? fminf(r[e] * 0x1p-100f, -0x1p-126f) : r[e];  // stays below 0
+    }
+  }
   x.scale = mb.byte | (rb.byte << 8);
-  if (mb.big) {
-#pragma unroll
-    for (int e = 0; e < 8; ++e) m[e] *= 0x1p-100f;
-  }
-  if (rb.big) {
-#pragma unroll
-    for (int e = 0; e < 8; ++e) r[e] = r[e] < 0.f ? fminf(r[e] * 0x1p-100f, -0x1p-126f) : r[e];  // stays below 0
-  }
   // place * multiplier + key, stepped from element to element
   const unsigned long long p0 = place + quant_at<VEC>(0);
   const unsigned first = (unsigned)p0 * kPlaceMul + (unsigned)(p0 >> 32) * kHighMul + a.key;
@@ -438,8 +448,11 @@ __device__ __forceinline__ void quant_step(QuantUnit &x, const AdamWArgs &a, flo
       for (int e = 0; e < 4; ++e)
         if (r[4 * q + e] < 0.f && ((rw >> (8 * e)) & 0xffu) == 0u) rw |= 1u << (8 * e);
     }
-    x.m[q] = mb.byte == 255u ? 0u : mw;
-    x.r[q] = rb.byte == 255u ? 0u : rw;
+    x.m[q] = mw, x.r[q] = rw;
+  }
+  if (unusual) {
+    if (mb.byte == 255u) x.m[0] = x.m[1] = 0u;
+    if (rb.byte == 255u) x.r[0] = x.r[1] = 0u;
   }
 }
 __device__ __forceinline__ void put_scale(const QuantUnit &x, unsigned char *scale) {
