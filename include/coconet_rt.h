@@ -337,11 +337,15 @@ int cocoFusedLAMBScattered(cocoComm_t comm, size_t nbuff, const void *const *g,
  *  - A tensor of 0 elements is allowed and its pointers are not looked at.
  *    Gradients, weights, copies and state must not overlap one another.
  *  - Elements need only the alignment of their type; tensors that start on 16
- *    bytes are faster.
+ *    bytes are faster.  The aligned 16 bytes in which a gradient or weight tensor
+ *    begins and ends may be read as a whole (not written).
  *  - World size 1: a call is one kernel per 1024 tensors and keeps nothing of the
  *    list, so it may be captured into a CUDA graph; the scalars are replayed as
  *    they were captured.  Above it a call that is being captured is refused
  *    (cocoInvalidUsage).
+ *  - AdamW calls of one communicator may overlap at world size 1; gradient norms
+ *    share its partial sums, like any two fused calls.  cocoLastPhaseTimes and
+ *    cocoLastCtaSpread do not cover these calls.
  *
  * cocoGradNormScattered:  norm[0] = |grad_scale| * || sum over ranks of g ||_2
  * over the whole list, norm[1] = max_norm / norm[0] where 0 < max_norm < norm[0]

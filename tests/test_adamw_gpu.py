@@ -789,3 +789,18 @@ def test_places_beyond_32_bits(comm, op):
             assert np.array_equal(st[2].view(torch.uint8)[(off + a) // 256].cpu().numpy(), out[3][0]), p
     assert (np.abs(w[at].cpu().numpy() - rw) <= 10 * A.U * np.abs(rw)).all()   # w = -q: near32
     assert int((w != 0).sum()) == 6
+
+
+def test_a_norm_longer_than_a_launch_counts(comm):
+    """2^31 groups of 16 bytes are one launch; the tensor ends 25 groups behind."""
+    torch.cuda.empty_cache()
+    n = (1 << 33) + 99
+    if torch.cuda.mem_get_info()[0] < 40 << 30:
+        pytest.skip("needs 40 GB of free device memory")
+    g = torch.zeros(n, device="cuda")
+    for at, x in ((0, 1.0), ((1 << 33) - 1, 2.0), (1 << 33, 4.0), (n - 1, 8.0)):
+        g[at] = x
+    out, before = torch.zeros(2, device="cuda"), comm.launch_count()
+    comm.grad_norm_scattered([g], out)
+    assert comm.launch_count() == before + 2
+    assert abs(float(out[0]) - math.sqrt(85.0)) <= 5.1 * A.U * math.sqrt(85.0)
