@@ -344,7 +344,11 @@ class TensorList:
             index = gs[0].get_device() if gs[0].is_cuda else None
             for what, ts, like in (("gradient", gs, gs[0].dtype), ("weight", ws, torch.float32),
                                    ("low-precision copy", lps, lps[0].dtype if lps else None)):
-                for k, (t, count) in enumerate(zip(ts or (), self.counts)):
+                T = torch.Tensor
+                if ts is None or (all(map(T.is_contiguous, ts)) and set(map(T.get_device, ts)) == {index} and
+                                  {t.dtype for t in ts} == {like} and list(map(T.numel, ts)) == self.counts[:]):
+                    continue
+                for k, (t, count) in enumerate(zip(ts, self.counts)):   # which one it is
                     if t.dtype != like:
                         raise ValueError(f"{what} {k} is {t.dtype}, not {like}")
                     if t.get_device() != index:
