@@ -29,7 +29,7 @@
 #define COCO_ADAMW_THREADS 352
 #endif
 #ifndef COCO_ADAMW_PACKED_THREADS
-#define COCO_ADAMW_PACKED_THREADS 256
+#define COCO_ADAMW_PACKED_THREADS 320
 #endif
 #ifndef COCO_ADAMW_QUANT_THREADS
 #define COCO_ADAMW_QUANT_THREADS 384
@@ -616,8 +616,10 @@ __global__ void __launch_bounds__(COCO_ADAMW_THREADS, 2)
 //  asynchronous copies by every warp for itself 1.20 ms (102 instructions per element),
 //  L2 prefetches one to three units ahead 1.02 to 1.07 ms.  Two tiles in flight 1.01,
 //  three 0.88, four 0.91 ms; 16, 14, 12, 11, 10 warps 0.91, 0.91, 0.88, 0.98, 0.91 ms.
-//  fp32 moments, 900 tensors, 29 M elements, hardly one aligned: 131 us (0.94) against
-//  146 us with element by element loads and stores.
+//  fp32 moments, 900 tensors, 29 M elements, hardly one aligned: 138 us (0.90) against
+//  146 us with element by element loads and stores; 30 such tensors of fp32 gradients,
+//  21 M elements: 101 us (0.94).  8 and 9 warps with three tiles in flight 141 and 146 us,
+//  10 and 12 warps, which leave room for two, 138 and 142 us.
 template <bool QUANT, typename GT> struct Pipe {
   static constexpr int kThreads = QUANT ? COCO_ADAMW_QUANT_THREADS : COCO_ADAMW_PACKED_THREADS, kCtas = 2;
   static constexpr int kWarps = kThreads / 32, kTile = kWarps * kListUnit;
