@@ -804,3 +804,55 @@ def test_a_norm_longer_than_a_launch_counts(comm):
     comm.grad_norm_scattered([g], out)
     assert comm.launch_count() == before + 2
     assert abs(float(out[0]) - math.sqrt(85.0)) <= 5.1 * A.U * math.sqrt(85.0)
+
+
+@pytest.mark.parametrize("hyper", [
+    dict(beta1=0.0, beta2=0.0), dict(beta1=0.5, beta2=0.125), dict(beta1=0.99, beta2=0.99999), dict(eps=0.0), dict(lr=0.0),
+    dict(weight_decay=0.0, eps=1e-8), dict(beta1=0.0, beta2=0.999, eps=1.0)])
+@pytest.mark.parametrize("scale", [1.0, 2.0 ** -44])
+def test_hyper_parameters_at_their_ends(comm, hyper, scale):
+    """Moments and codes bit for bit, weights near, for betas of 0 and near 1, no eps, no lr, and for gradients whose
+    squares lie below the fp32 normal range."""
+    h = {k: A.F(v) for k, v in dict(A.HYPER, **hyper).items()}
+    n = 3000
+    r = np.random.default_rng(11)
+    g = (r.normal(0, 1e-3, n) * scale).astype(np.float32)
+    g[g == 0] = np.float32(1e-3 * scale)
+    w0 = r.normal(0, 0.02, n).astype(np.float32)
+    args = [float(h[k]) for k in ("lr", "beta1", "beta2", "eps", "weight_decay")]
+    gd = torch.from_numpy(g).cuda()
+    w, m, v = torch.from_numpy(w0.copy()).cuda(), torch.zeros(n, device="cuda"), torch.zeros(n, device="cuda")
+    q, st = torch.from_numpy(w0.copy()).cuda(), coco.quant_state([n], 1)
+    om, ov, ow = np.zeros(n, np.float32), np.zeros(n, np.float32), w0.copy()
+    mc, rc, sc = np.zeros(n, np.uint8), np.zeros(n, np.uint8), np.zeros((12, 2), np.uint8)
+    for step in range(3):
+        comm.fused_adamw_scattered([gd], [w], m, v, *args, step)
+        comm.fused_adamw_quant_scattered([gd], [q], *st, *args, step, 4)
+        before = (ow, om, ov, g)
+        _, om, ov = A.step32(*before, step, hyper=h)
+        assert np.array_equal(m.cpu().numpy(), om) and np.array_equal(v.cpu().numpy(), ov), step
+        ow = w.cpu().numpy().copy()
+        if scale == 1.0:   # (below, the root of a number without a normal range has no relative bound)
+            assert A.near32(ow, *before, step, hyper=h), step
+        out = A.quant_step32(w0, mc, rc, sc, g, step, 4, 0, hyper=h)
+        _, mc, rc, sc = out[:4]
+        assert np.array_equal(st[0].view(torch.uint8).cpu().numpy()[:n], mc), step
+        assert np.array_equal(st[1].view(torch.uint8).cpu().numpy()[:n], rc), step
+        assert np.array_equal(st[2].view(torch.uint8).cpu().numpy(), sc), step
+        assert bool(torch.isfinite(q).all()), step
+
+
+def test_fewer_ctas_give_the_same_step(comm):
+    counts = RAGGED + [300001]
+    w, m, v, (g,) = _make(counts, 80, "bf16")
+    results = []
+    for ctas in (0, 1):
+        comm.set_tunables(ctas_per_sm=ctas)
+        gs, ws, qs = _aligned(g, torch.bfloat16), _aligned(w, torch.float32), _views(w, torch.float32, 1, 0)[1]
+        st, qst, norm = [torch.from_numpy(_flat(x, counts, 8)).cuda() for x in (m, v)], coco.quant_state(counts, 1), torch.zeros(2, device="cuda")
+        comm.grad_norm_scattered(gs, norm, max_norm=0.01)
+        assert abs(float(norm[0]) - _norm64(g)) <= 5.1 * A.U * _norm64(g)
+        comm.fused_adamw_scattered(gs, ws, *st, H["lr"], H["beta1"], H["beta2"], H["eps"], 0.1, 3)
+        comm.fused_adamw_quant_scattered(gs, qs, *qst, H["lr"], H["beta1"], H["beta2"], H["eps"], 0.1, 3, 2)
+        results.append(ws + qs + st + [x.view(torch.uint8) for x in qst])
+    assert all(torch.equal(a, b) for a, b in zip(*results))
