@@ -24,7 +24,7 @@
 
 #include <atomic>
 
-// Threads of a CTA, two CTAs per SM, and tiles in flight of the staged kernels.
+// Threads of a CTA where an SM holds two, and tiles in flight of the staged kernels.
 #ifndef COCO_ADAMW_THREADS
 #define COCO_ADAMW_THREADS 352
 #endif
@@ -611,17 +611,19 @@ __global__ void __launch_bounds__(COCO_ADAMW_THREADS, 2)
 // below its start to the one above its end (memory of the same allocation), and its new
 // weights leave through shared memory, in 16-byte stores but for the ends of a unit.
 // Where a tile holds several tensors its units are copied one by one.
-//  8-bit moments, 336 M elements (16 bytes each): 0.88 ms, 0.93 of the copy rate, in a
-//  burst, 0.92 ms at the clocks of a long run; loads by the threads themselves 0.94 ms,
-//  asynchronous copies by every warp for itself 1.20 ms (102 instructions per element),
-//  L2 prefetches one to three units ahead 1.02 to 1.07 ms.  Two tiles in flight 1.01,
-//  three 0.88, four 0.91 ms; 16, 14, 12, 11, 10 warps 0.91, 0.91, 0.88, 0.98, 0.91 ms.
+//  8-bit moments, 336 M elements (16 bytes each): 0.83 ms, 0.99 of the copy rate, in a
+//  burst, 0.92 ms at the clocks of a long run; with four tiles in flight in place of three
+//  0.92.  With two CTAs per SM 0.88 ms in a burst, and beside that: loads by the threads
+//  themselves 0.94 ms, asynchronous copies by every warp for itself 1.20 ms (102
+//  instructions per element), L2 prefetches one to three units ahead 1.02 to 1.07 ms; two
+//  tiles in flight 1.01, four 0.91 ms; 16, 14, 11, 10 warps 0.91, 0.91, 0.98, 0.91 ms.
 //  fp32 moments, 900 tensors, 29 M elements, hardly one aligned: 138 us (0.90) against
 //  146 us with element by element loads and stores; 30 such tensors of fp32 gradients,
 //  21 M elements: 101 us (0.94).  8 and 9 warps with three tiles in flight 141 and 146 us,
 //  10 and 12 warps, which leave room for two, 138 and 142 us.
-template <bool QUANT, typename GT> struct Pipe {
-  static constexpr int kThreads = QUANT ? COCO_ADAMW_QUANT_THREADS : COCO_ADAMW_PACKED_THREADS, kCtas = 2;
+template <bool QUANT, bool WIDE, typename GT> struct Pipe {
+  static constexpr int kThreads = !QUANT ? COCO_ADAMW_PACKED_THREADS : WIDE ? 2 * COCO_ADAMW_QUANT_THREADS : COCO_ADAMW_QUANT_THREADS;
+  static constexpr int kCtas = WIDE ? 1 : 2;  // of an SM
   static constexpr int kWarps = kThreads / 32, kTile = kWarps * kListUnit;
   static constexpr int kState = kTile * (QUANT ? 1 : 4);  // bytes of m and of v
   // the gradients and weights of a tile, or of its units one by one
@@ -630,8 +632,8 @@ template <bool QUANT, typename GT> struct Pipe {
   static constexpr int kV = kM + kState, kScale = kV + kState;
   static constexpr int kBytes = kScale + (QUANT ? (kWarps * 2 + 15) / 16 * 16 + 16 : 0);
   static constexpr int kLp = kWarps * (kListUnit * 2 + 16);  // copies on their way out
-  // of an SM's 228 KB: 1 KB per CTA is reserved, 7 KB are the kernel's other tables
-  static constexpr int kFit = ((228 * 1024) / kCtas - 8 * 1024 - kLp) / kBytes;
+  // of an SM's 228 KB: 1 KB per CTA is reserved, up to 9 KB are the kernel's other tables
+  static constexpr int kFit = ((228 * 1024) / kCtas - 10 * 1024 - kLp) / kBytes;
   static constexpr int kStages = kFit < COCO_ADAMW_STAGES ? kFit : COCO_ADAMW_STAGES;
   static_assert(kStages >= 2 && kBytes % 16 == 0, "a tile is loaded while another is worked on");
   static constexpr int kSmem = kStages * kBytes + kLp;
@@ -670,10 +672,11 @@ struct __align__(16) UnitInfo {
   static constexpr unsigned kDecays = 1u << 16;
 };
 
-template <bool QUANT, typename GT, int CAP>
-__global__ void __launch_bounds__((Pipe<QUANT, GT>::kThreads), (Pipe<QUANT, GT>::kCtas))
+template <bool QUANT, bool WIDE, typename GT, int CAP>
+__global__ void __launch_bounds__((Pipe<QUANT, WIDE, GT>::kThreads), (Pipe<QUANT, WIDE, GT>::kCtas))
     adamw_staged_kernel(const __grid_constant__ ListTable<CAP> tab, const __grid_constant__ AdamWArgs a) {
-  typedef Pipe<QUANT, GT> P;
+  typedef Pipe<QUANT, WIDE, GT> P;
+  static_assert(P::kWarps <= 32, "a lane of the asking warp looks after each unit");
   constexpr unsigned S = P::kStages, kTileGroups = P::kTile / kListGroup;
   extern __shared__ __align__(128) unsigned char s_stage[];
   __shared__ unsigned s_off[CAP + 1];
@@ -978,25 +981,26 @@ template <int CAP> using Kernel = void (*)(const ListTable<CAP>, const AdamWArgs
 struct LaunchShape {
   int threads, ctas_per_sm, smem;
 };
-template <bool STAGED, bool QUANT, typename GT, int CAP> Kernel<CAP> pick_one(LaunchShape *sh) {
-  if constexpr (STAGED) {
-    typedef Pipe<QUANT, GT> P;
-    *sh = {P::kThreads, P::kCtas, P::kSmem};
-    return adamw_staged_kernel<QUANT, GT, CAP>;
-  } else {
-    *sh = {COCO_ADAMW_THREADS, 2, 0};
-    return adamw_kernel<GT, CAP>;
-  }
+template <bool QUANT, bool WIDE, typename GT, int CAP> Kernel<CAP> pick_staged(LaunchShape *sh) {
+  typedef Pipe<QUANT, WIDE, GT> P;
+  *sh = {P::kThreads, P::kCtas, P::kSmem};
+  return adamw_staged_kernel<QUANT, WIDE, GT, CAP>;
 }
-// 8-bit moments: staged tiles, which measured better for aligned tensors too.  fp32
-// moments: staged tiles where tensors are not aligned, which the direct kernel would
+// 8-bit moments: staged tiles, which measured better for aligned tensors too.  `wide`,
+// one CTA of 24 warps per SM in place of two of 12, has half as many tiles: better where
+// they lie in one tensor mostly (398 tensors, 336 M elements: 0.83 against 0.88 ms; 30
+// tensors, 21 M: 56.5 against 57.5 us), worse where many hold several (900 tensors, 29 M:
+// 84 against 80 us, packed 102 against 96).
+// fp32 moments: staged tiles where tensors are not aligned, which the direct kernel would
 // walk element by element; else the direct kernel (12.6 M elements 58 against 61 us,
 // 336 M 1.49 against 1.51 ms).
-template <int CAP> Kernel<CAP> pick(bool quant, bool packed, cocoDataType_t g, LaunchShape *sh) {
+template <int CAP> Kernel<CAP> pick(bool quant, bool packed, bool wide, cocoDataType_t g, LaunchShape *sh) {
   auto of = [&](auto type) -> Kernel<CAP> {
     typedef decltype(type) GT;
-    return quant ? pick_one<true, true, GT, CAP>(sh)
-           : packed ? pick_one<true, false, GT, CAP>(sh) : pick_one<false, false, GT, CAP>(sh);
+    if (quant) return wide ? pick_staged<true, true, GT, CAP>(sh) : pick_staged<true, false, GT, CAP>(sh);
+    if (packed) return pick_staged<false, false, GT, CAP>(sh);
+    *sh = {COCO_ADAMW_THREADS, 2, 0};
+    return adamw_kernel<GT, CAP>;
   };
   switch (g) {
     case cocoFloat32: return of(float());
@@ -1005,6 +1009,8 @@ template <int CAP> Kernel<CAP> pick(bool quant, bool packed, cocoDataType_t g, L
   }
   return nullptr;
 }
+// Units per tensor, on average, from which on `wide` is taken: 256 Ki elements.
+constexpr size_t kWideUnits = 1024;
 typedef void (*PeerKernel)(const PeerArgs, const AdamWArgs);
 template <bool QUANT, typename GT> PeerKernel pick_world(int world) {
   return world <= 2 ? adamw_peer_kernel<QUANT, GT, 2>
@@ -1032,11 +1038,12 @@ cudaError_t launch_adamw(bool quant, bool packed, cocoDataType_t g_type, const L
                          const AdamWArgs &args, size_t units, int device, int sm_count,
                          int max_ctas_per_sm, cudaStream_t stream) {
   LaunchShape sh;
-  const Kernel<CAP> k = pick<CAP>(quant, packed, g_type, &sh);
+  const bool wide = quant && units >= kWideUnits * (size_t)args.n;
+  const Kernel<CAP> k = pick<CAP>(quant, packed, wide, g_type, &sh);
   if (!k) return cudaErrorInvalidValue;
   if (sh.smem > 0) {  // more than the default: allowed once per kernel and device
-    static std::atomic<unsigned long long> allowed[2][3];
-    std::atomic<unsigned long long> &mask = allowed[quant][g_type == cocoFloat32 ? 0 : g_type == cocoFloat16 ? 1 : 2];
+    static std::atomic<unsigned long long> allowed[2][2][3];
+    std::atomic<unsigned long long> &mask = allowed[quant][wide][g_type == cocoFloat32 ? 0 : g_type == cocoFloat16 ? 1 : 2];
     const unsigned long long bit = device < 64 ? 1ull << device : 0;
     if (!(mask.load(std::memory_order_acquire) & bit)) {
       const cudaError_t e = cudaFuncSetAttribute((const void *)k, cudaFuncAttributeMaxDynamicSharedMemorySize, sh.smem);

@@ -856,3 +856,53 @@ def test_fewer_ctas_give_the_same_step(comm):
         comm.fused_adamw_quant_scattered(gs, qs, *qst, H["lr"], H["beta1"], H["beta2"], H["eps"], 0.1, 3, 2)
         results.append(ws + qs + st + [x.view(torch.uint8) for x in qst])
     assert all(torch.equal(a, b) for a, b in zip(*results))
+
+
+@pytest.mark.parametrize("gt,lp", [("f32", "f16"), ("f16", "f16"), ("bf16", None)])
+@pytest.mark.parametrize("packed", [False, True])
+def test_quant_adamw_of_large_tensors_bit_for_bit(comm, gt, lp, packed):
+    """Lists of 1024 and more units a tensor, on average, with small tensors and ragged ends among them."""
+    counts = [900001, 17, 300000, 256, 40960 * 6]
+    assert sum(-(-c // 256) for c in counts) >= 1024 * len(counts)
+    off, total = A.starts(counts, 256)[0], coco.quant_slice_elems(counts, 1)
+    w, m, v, (g,) = _make(counts, 90, gt)
+    state = _quant_initial(counts, m, v, 91)
+    mf, rf, sf = np.full(total, 0x55, np.uint8), np.full(total, 0x55, np.uint8), np.full((total // 256, 2), 0x44, np.uint8)
+    for o, (mc, rc, sc) in zip(off, state):
+        mf[o:o + mc.size], rf[o:o + rc.size], sf[o // 256:o // 256 + len(sc)] = mc, rc, sc
+    st = [torch.from_numpy(x.copy()).cuda() for x in (mf, rf, sf)]
+    bufs = {}
+
+    def place(name, arrays, dtype):
+        if not packed:
+            return _aligned(arrays, dtype)
+        bufs[name] = _views(arrays, dtype, 1, 3)
+        return bufs[name][1]
+    gs, ws = place("g", g, TYPES[gt]), place("w", w, torch.float32)
+    lps = place("lp", [np.zeros(c, np.float32) for c in counts], TYPES[lp]) if lp else None
+    no_decay = [False, True, True, False, False]
+    for step in (2, 3):
+        comm.fused_adamw_quant_scattered(gs, ws, *st, H["lr"], H["beta1"], H["beta2"], H["eps"], H["weight_decay"], step, 77,
+                                         w_lps=lps, no_decay=no_decay)
+        gm, gr, gsc = (x.cpu().numpy() for x in st)
+        for b, c in enumerate(counts):
+            mc, rc, sc = state[b]
+            old = (A.code_values(mc) * A.scale_values(sc[:, 0]).repeat(256)[:c],
+                   (A.code_values(rc) * A.scale_values(sc[:, 1]).repeat(256)[:c]) ** 2)
+            _, mc, rc, sc, _, _ = A.quant_step32(w[b], mc, rc, sc, g[b], step, 77, off[b], not no_decay[b])
+            state[b] = (mc, rc, sc)
+            assert np.array_equal(gm[off[b]:off[b] + c], mc), (step, b)
+            assert np.array_equal(gr[off[b]:off[b] + c], rc), (step, b)
+            assert np.array_equal(gsc[off[b] // 256:off[b] // 256 + len(sc)], sc), (step, b)
+            before, now = w[b].astype(np.float64), ws[b].cpu().numpy()
+            x = (before, old[0], old[1], g[b].astype(np.float64), step, not no_decay[b])
+            assert (np.abs(now - A.step64(*x)[0]) <= A.bounds64(*x)[0]).all(), (step, b)
+            w[b] = now
+            if lp:
+                assert np.array_equal(lps[b].float().cpu().numpy(), _lp_of(now, lp)), (step, b)
+    assert all(_gaps_untouched(*x) for x in bufs.values())
+    used = np.zeros(total, bool)
+    for o, c in zip(off, counts):
+        used[o:o + c] = True
+    gm, gr, _ = (x.cpu().numpy() for x in st)
+    assert (gm[~used] == 0x55).all() and (gr[~used] == 0x55).all()
