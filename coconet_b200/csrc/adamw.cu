@@ -990,7 +990,8 @@ template <bool QUANT, bool WIDE, typename GT, int CAP> Kernel<CAP> pick_staged(L
 // one CTA of 24 warps per SM in place of two of 12, has half as many tiles: better where
 // they lie in one tensor mostly (398 tensors, 336 M elements: 0.83 against 0.88 ms; 30
 // tensors, 21 M: 56.5 against 57.5 us), worse where many hold several (900 tensors, 29 M:
-// 84 against 80 us, packed 102 against 96).
+// 84 against 80 us, packed 102 against 96) and on few tiles (one tensor of 256 Ki elements
+// 5.0 against 3.8 us, of 1 Mi 7.4 against 6.0; of 4 Mi the same, of 16 Mi 46.6 against 47.1).
 // fp32 moments: staged tiles where tensors are not aligned, which the direct kernel would
 // walk element by element; else the direct kernel (12.6 M elements 58 against 61 us,
 // 336 M 1.49 against 1.51 ms).
@@ -1009,8 +1010,9 @@ template <int CAP> Kernel<CAP> pick(bool quant, bool packed, bool wide, cocoData
   }
   return nullptr;
 }
-// Units per tensor, on average, from which on `wide` is taken: 256 Ki elements.
-constexpr size_t kWideUnits = 1024;
+// From how many units per tensor, on average, and per SM `wide` is taken: 256 Ki elements
+// a tensor, 8 tiles a CTA.
+constexpr size_t kWideUnits = 1024, kWideUnitsPerSm = 8 * 2 * COCO_ADAMW_QUANT_THREADS / 32;
 typedef void (*PeerKernel)(const PeerArgs, const AdamWArgs);
 template <bool QUANT, typename GT> PeerKernel pick_world(int world) {
   return world <= 2 ? adamw_peer_kernel<QUANT, GT, 2>
@@ -1038,7 +1040,7 @@ cudaError_t launch_adamw(bool quant, bool packed, cocoDataType_t g_type, const L
                          const AdamWArgs &args, size_t units, int device, int sm_count,
                          int max_ctas_per_sm, cudaStream_t stream) {
   LaunchShape sh;
-  const bool wide = quant && units >= kWideUnits * (size_t)args.n;
+  const bool wide = quant && units >= kWideUnits * (size_t)args.n && units >= kWideUnitsPerSm * (size_t)sm_count;
   const Kernel<CAP> k = pick<CAP>(quant, packed, wide, g_type, &sh);
   if (!k) return cudaErrorInvalidValue;
   if (sh.smem > 0) {  // more than the default: allowed once per kernel and device

@@ -861,9 +861,10 @@ def test_fewer_ctas_give_the_same_step(comm):
 @pytest.mark.parametrize("gt,lp", [("f32", "f16"), ("f16", "f16"), ("bf16", None)])
 @pytest.mark.parametrize("packed", [False, True])
 def test_quant_adamw_of_large_tensors_bit_for_bit(comm, gt, lp, packed):
-    """Lists of 1024 and more units a tensor, on average, with small tensors and ragged ends among them."""
-    counts = [900001, 17, 300000, 256, 40960 * 6]
-    assert sum(-(-c // 256) for c in counts) >= 1024 * len(counts)
+    """Lists of 1024 and more units a tensor, on average, and of 8 tiles and more a CTA, with small tensors and ragged ends among them."""
+    counts = [900001, 17, 5300000, 256, 40960 * 40]
+    sms = torch.cuda.get_device_properties(0).multi_processor_count
+    assert sum(-(-c // 256) for c in counts) >= max(1024 * len(counts), 8 * 24 * sms)
     off, total = A.starts(counts, 256)[0], coco.quant_slice_elems(counts, 1)
     w, m, v, (g,) = _make(counts, 90, gt)
     state = _quant_initial(counts, m, v, 91)
