@@ -197,7 +197,9 @@ __global__ void __launch_bounds__(COCO_NORM_THREADS)
   const PeerPiece *pieces = pr.pieces;
   const unsigned units = started ? (pr.groups + kListUnitGroups - 1) / kListUnitGroups : 0;
   const unsigned nw = blockDim.x >> 5;
-  double sum = 0.0;
+  // Every CTA waits for itself, and some may have given up where others, which came
+  // later, did not: a sum without their part is no number, on every rank.
+  double sum = started ? 0.0 : __longlong_as_double(0x7ff8000000000000ll);
   auto add = [&](float x) { sum += (double)x * (double)x; };
   for (unsigned u = blockIdx.x * nw + (threadIdx.x >> 5); u < units; u += gridDim.x * nw) {
     const unsigned e = u * kListUnitGroups;
