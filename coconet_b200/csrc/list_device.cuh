@@ -108,25 +108,29 @@ __device__ __forceinline__ bool list_start_barrier(const PeerRank &pr, const Pee
 }
 // The rank's last CTA announces that its reads and writes are complete and
 // waits for the others', so that the kernel ends only when nobody touches this
-// rank's memory any more.
+// rank's memory any more.  Where a CTA of the rank gave up at the start (ok), its
+// part is missing: nothing is announced, and the other ranks' waits run out, so
+// that their status words say so too.
 __device__ __forceinline__ void list_end_barrier(const PeerRank &pr, const PeerArgs &pa, bool ok) {
+  constexpr unsigned kGaveUp = 0x10000u;  // in the counter's upper half: CTAs that did
+  static_assert(kMaxCtasPerRank < kGaveUp, "a rank's CTAs are counted in 16 bits");
   FlagPage *me = pr.flags[pr.rank];
   __threadfence_system();
   __syncthreads();
   if (threadIdx.x >= 32) return;
-  unsigned prev = 0;
+  unsigned ctas = 0;
   if (threadIdx.x == 0) {
+    const unsigned mine = ok ? 1u : 1u + kGaveUp;
     __threadfence_system();
-    prev = atomicAdd(&me->done_count, 1u);
-    if (prev == gridDim.x - 1) me->done_count = 0;
+    ctas = atomicAdd(&me->done_count, mine) + mine;
+    if (ctas % kGaveUp == gridDim.x) me->done_count = 0;
     __threadfence_system();
   }
   __syncwarp();
-  prev = __shfl_sync(0xffffffffu, prev, 0);
-  if (prev != gridDim.x - 1) return;
+  ctas = __shfl_sync(0xffffffffu, ctas, 0);
+  if (ctas != gridDim.x) return;  // not the last, or not complete
   __threadfence_system();
   warp_signal_peers(pr, pa.world, pr.rank, pa.seq, [](FlagPage *f) { return f->done; });
-  if (!ok) return;
   const int late = warp_wait_peers(me->done, pa.world, pr.rank, pa.seq, pa.timeout_ns);
   if (late >= 0 && threadIdx.x == 0)
     record_status(me, cocoTimeout, pr.rank, kPhaseEnd, late, pa.seq);

@@ -1,6 +1,7 @@
 """A rank whose CTAs disagree on whether a peer came in time (tests/late_rank.cu): the
-part of a gradient norm that is missing must not pass for a norm.  CPU: the program
-compiles for sm_100a against the library.  GPU: every wait in it is bounded."""
+part of a gradient norm that is missing must not pass for a norm, and a step that is
+missing a part must not be announced as complete.  CPU: the program compiles for
+sm_100a against the library.  GPU: every wait in it is bounded."""
 import json
 import os
 import subprocess
@@ -53,3 +54,19 @@ def test_norm_that_lost_a_part_is_no_number(program):
     assert out["norm"] != out["norm"] and out["clip"] == 0.0, out   # nan: the step that reads it is skipped
     if out["told_norm"]:           # what the peer adds up is no number either
         assert out["told_part"] != out["told_part"], out
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("op", ["adamw", "adamw8"])
+def test_step_with_a_rank_in_time(program, op):
+    out = _run(program, op, "in-time")
+    assert out["status"] == 0 and out["stepped"] == out["n"] and out["told_done"] == 1
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("op", ["adamw", "adamw8"])
+def test_step_that_lost_a_part_is_not_announced_as_done(program, op):
+    out = _run(program, op)
+    assert out["status"] == 5 and out["phase"] == 1
+    assert 0 < out["stepped"] < out["n"], out   # some CTAs gave up, others did not
+    assert out["told_done"] == 0, out           # the peer's wait runs out: its status says so too
