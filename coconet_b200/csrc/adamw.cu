@@ -217,26 +217,22 @@ __device__ __forceinline__ void scales_of(unsigned bytes, float &lo, float &hi) 
 // A block's scale byte and what to multiply its values by before they are rounded,
 // from the largest magnitude (as bits) of the block: the largest code lies in
 // [128, 256), which leaves room to round up below 448.  255 (not a number): the block
-// holds inf or nan.  The factor, 2^(7 - e - 120), is no float for the largest e: `big`
-// says that the values are to be multiplied by 2^-100 first.
+// holds inf or nan.  The product of the two factors, 2^(14 - e) for a largest exponent
+// field of e, is no float for the largest e; the first leaves the largest value in
+// [2^7, 2^8) and costs nothing but what is far below the smallest code.
 struct BlockScale {
   unsigned byte;
-  bool big;
-  float factor;
+  float before, factor;
 };
 __device__ __forceinline__ BlockScale block_scale(unsigned max_bits) {
   unsigned e = max_bits >> 23;
   e = e < 8u ? 8u : e > 254u ? 254u : e;
-  BlockScale b;
-  b.byte = max_bits >= 0x7f800000u ? 255u : e - 7u;
-  b.big = e > 140u;
-  b.factor = __uint_as_float((141u - (b.big ? e - 100u : e)) << 23);
-  return b;
+  return {max_bits >= 0x7f800000u ? 255u : e - 7u, __uint_as_float((261u - e) << 23), 0x1p-120f};
 }
-// The same where the largest magnitude lies in [2^-119, 2^14).
+// The same where the largest magnitude lies in [2^-119, 2^14): one factor does.
 __device__ __forceinline__ bool is_usual(unsigned max_bits) { return max_bits - 0x04000000u < 0x46800000u - 0x04000000u; }
 __device__ __forceinline__ BlockScale usual_scale(unsigned max_bits) {
-  return {(max_bits >> 23) - 7u, false, __uint_as_float(0x46800000u - (max_bits & 0x7f800000u))};
+  return {(max_bits >> 23) - 7u, 1.f, __uint_as_float(0x46800000u - (max_bits & 0x7f800000u))};
 }
 // x times the block's factor has the code's 7 magnitude bits in bits 20..26, subnormal
 // codes included; adding 20 random bits (16 of the hash, a one that centres them, zeros)
@@ -423,13 +419,10 @@ __device__ __forceinline__ void quant_step(QuantUnit &x, const AdamWArgs &a, flo
   const bool unusual = !is_usual(m_top) || !is_usual(r_top);
   if (unusual) {
     mb = block_scale(m_top), rb = block_scale(r_top);
-    if (mb.big) {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) m[e] *= 0x1p-100f;
-    }
-    if (rb.big) {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) r[e] = r[e] < 0.f ? fminf(r[e] * 0x1p-100f, -0x1p-126f) : r[e];  // stays below 0
+    for (int e = 0; e < 8; ++e) {
+      m[e] *= mb.before;
+      r[e] = r[e] < 0.f ? fminf(r[e] * rb.before, -0x1p-126f) : r[e];  // stays below 0
     }
   }
   x.scale = mb.byte | (rb.byte << 8);
