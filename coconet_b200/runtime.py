@@ -554,6 +554,19 @@ class Communicator:
         return stream.cuda_stream if stream is not None else torch._C._cuda_getCurrentRawStream(device)
 
     @staticmethod
+    def _list_of(gs, ws, w_lps, no_decay):
+        """The list of an AdamW call.  A TensorList brings its own weights, copies and
+        no_decay; others beside it would have no place to go."""
+        if not isinstance(gs, TensorList):
+            return TensorList(gs, ws, w_lps, no_decay)
+        for what, given, own in (("ws", ws, gs.tensors[1]), ("w_lps", w_lps, gs.tensors[2])):
+            if given is not None and (own is None or len(given) != gs.n or any(a is not b for a, b in zip(given, own))):
+                raise ValueError(f"a TensorList holds its own tensors; {what} has to be None or the same beside it")
+        if no_decay is not None and [bool(x) for x in no_decay] != [bool(x) for x in gs.no_decay or [0] * gs.n]:
+            raise ValueError("a TensorList holds its own switches; no_decay has to be None or the same beside it")
+        return gs
+
+    @staticmethod
     def _held(t, what, device, dtypes, least):
         """Pointer of a state tensor after a look at its type and size."""
         if t.dtype not in dtypes or t.get_device() != device or not t.is_contiguous() or t.numel() < least:
@@ -577,9 +590,10 @@ class Communicator:
                               w_lps=None, no_decay=None, grad_scale=1.0, norm=None, stream=None):
         """AdamW over a list, fp32 moments.  `norm`: as grad_norm_scattered left it;
         the gradients are scaled by norm[1], and a norm that is not finite skips
-        the step.  With a TensorList, its copies and no_decay apply."""
+        the step.  A TensorList brings its weights, copies and no_decay; other `ws`,
+        `w_lps` or `no_decay` beside it are refused."""
         import torch
-        lst = gs if isinstance(gs, TensorList) else TensorList(gs, ws, w_lps, no_decay)
+        lst = self._list_of(gs, ws, w_lps, no_decay)
         device = lst._checked(weights=True)
         need, f32 = lst._slice(self.world, False), (torch.float32,)
         g, w, lp, counts, no_decay = lst._at
@@ -594,9 +608,9 @@ class Communicator:
                                     step, seed, w_lps=None, no_decay=None, grad_scale=1.0, norm=None,
                                     stream=None):
         """AdamW over a list with 8-bit moments (see quant_state): e4m3 codes of m
-        and sqrt(v), rounded at random from `seed` and `step`."""
+        and sqrt(v), rounded at random from `seed` and `step`.  A TensorList as above."""
         import torch
-        lst = gs if isinstance(gs, TensorList) else TensorList(gs, ws, w_lps, no_decay)
+        lst = self._list_of(gs, ws, w_lps, no_decay)
         device = lst._checked(weights=True)
         need = lst._slice(self.world, True)
         code, exponent = (torch.float8_e4m3fn, torch.uint8), (torch.float8_e8m0fnu, torch.uint8)
