@@ -82,9 +82,10 @@ __device__ __forceinline__ double warp_sum(double x) {
   return x;
 }
 
-// The CTAs' sums, by the CTA that arrives last; true in that CTA only, with the
-// total in thread 0.
-__device__ __forceinline__ bool rank_sum(double x, FlagPage *page, double &total) {
+// The CTAs' sums (part, STRIDE apart), by the CTA that arrives last; true in that CTA
+// only, with the total in thread 0.
+template <int STRIDE>
+__device__ __forceinline__ bool rank_sum(double x, unsigned *count, double *part, double &total) {
   __shared__ double s_part[32];
   __shared__ int s_last;
   const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5, nw = blockDim.x >> 5;
@@ -95,9 +96,9 @@ __device__ __forceinline__ bool rank_sum(double x, FlagPage *page, double &total
     if (wid == 0) {
       x = warp_sum(lane < nw ? s_part[lane] : 0.0);
       if (lane == 0) {
-        page->cta_part[blockIdx.x][0] = x;
+        part[(size_t)blockIdx.x * STRIDE] = x;
         __threadfence();
-        s_last = atomicAdd(&page->norm_count, 1u) == gridDim.x - 1;
+        s_last = atomicAdd(count, 1u) == gridDim.x - 1;
       }
     }
     __syncthreads();
@@ -105,12 +106,12 @@ __device__ __forceinline__ bool rank_sum(double x, FlagPage *page, double &total
     __threadfence();
     x = 0.0;
     for (unsigned c = threadIdx.x; c < gridDim.x; c += blockDim.x)
-      x += ld_volatile_f64(&page->cta_part[c][0]);
+      x += ld_volatile_f64(&part[(size_t)c * STRIDE]);
     x = warp_sum(x);
     __syncthreads();
     if (lane == 0) s_part[wid] = x;
     __syncthreads();
-    if (threadIdx.x == 0) page->norm_count = 0;
+    if (threadIdx.x == 0) *count = 0;
   }
   total = wid == 0 ? warp_sum(lane < nw ? s_part[lane] : 0.0) : 0.0;
   return true;
@@ -129,7 +130,7 @@ __device__ __forceinline__ void put_norm(const NormArgs &a, float *out, double t
 template <typename GT, int CAP>
 __global__ void __launch_bounds__(COCO_NORM_THREADS, COCO_NORM_CTAS)
     norm_kernel(const __grid_constant__ NormTable<CAP> tab, const __grid_constant__ NormArgs a,
-                FlagPage *page) {
+                NormSlot *slot) {
   __shared__ unsigned s_off[CAP + 1];
   const NormTable<CAP> *tp = &tab;
   hide(tp);  // for lookups that differ from lane to lane
@@ -178,12 +179,10 @@ __global__ void __launch_bounds__(COCO_NORM_THREADS, COCO_NORM_CTAS)
     for (int k = 0; k < kDepth; ++k) sum += squares<GT>(q[k]);
   }
   double all = 0.0;
-  if (!rank_sum(sum, page, all) || threadIdx.x != 0) return;
-  // a list of several launches: the sum so far waits in a word of the page that
-  // world size 1 does not use between calls
-  if (!a.first) all += ld_volatile_f64(&page->norm_part[0][0]);
+  if (!rank_sum<1>(sum, &slot->count, reinterpret_cast<double *>(slot + 1), all) || threadIdx.x != 0) return;
+  if (!a.first) all += ld_volatile_f64(&slot->so_far);
   if (a.last) put_norm(a, a.out, all);
-  else page->norm_part[0][0] = all;
+  else slot->so_far = all;
 }
 
 template <typename GT, int RB>
@@ -227,7 +226,7 @@ __global__ void __launch_bounds__(COCO_NORM_THREADS)
     __syncwarp();
   }
   double all = 0.0;
-  if (!rank_sum(sum, me, all)) return;
+  if (!rank_sum<2>(sum, &me->norm_count, &me->cta_part[0][0], all)) return;
   // The rank's last CTA: nothing of this rank reads gradients any more.  Its sum
   // goes to every rank, and the others' arrival says the same of them.
   if (threadIdx.x >= 32) return;
@@ -252,7 +251,7 @@ __global__ void __launch_bounds__(COCO_NORM_THREADS)
   }
 }
 
-template <int CAP> using Kernel = void (*)(const NormTable<CAP>, const NormArgs, FlagPage *);
+template <int CAP> using Kernel = void (*)(const NormTable<CAP>, const NormArgs, NormSlot *);
 template <int CAP> Kernel<CAP> pick(cocoDataType_t g) {
   switch (g) {
     case cocoFloat32: return norm_kernel<float, CAP>;
@@ -282,16 +281,16 @@ int grad_norm_groups_per_warp() { return kUnit; }
 
 template <int CAP>
 cudaError_t launch_grad_norm(cocoDataType_t g_type, const NormTable<CAP> &table,
-                             const NormArgs &args, FlagPage *page, int ctas, cudaStream_t stream) {
+                             const NormArgs &args, NormSlot *slot, int ctas, cudaStream_t stream) {
   const Kernel<CAP> k = pick<CAP>(g_type);
   if (!k) return cudaErrorInvalidValue;
-  void *params[] = {(void *)&table, (void *)&args, (void *)&page};
+  void *params[] = {(void *)&table, (void *)&args, (void *)&slot};
   return cudaLaunchKernel((const void *)k, dim3(ctas), dim3(COCO_NORM_THREADS), params, 0, stream);
 }
 template cudaError_t launch_grad_norm<kNormCapSmall>(cocoDataType_t, const NormTable<kNormCapSmall> &,
-                                                     const NormArgs &, FlagPage *, int, cudaStream_t);
+                                                     const NormArgs &, NormSlot *, int, cudaStream_t);
 template cudaError_t launch_grad_norm<kNormCapLarge>(cocoDataType_t, const NormTable<kNormCapLarge> &,
-                                                     const NormArgs &, FlagPage *, int, cudaStream_t);
+                                                     const NormArgs &, NormSlot *, int, cudaStream_t);
 
 cudaError_t launch_grad_norm_peers(cocoDataType_t g_type, const PeerArgs &peers, const NormArgs &args,
                                    const ListLaunch &cfg, cudaStream_t stream) {

@@ -92,6 +92,12 @@ template <int CAP> struct NormTable {
   unsigned off[CAP + 1];               // first group; [n]: one past the last
   unsigned char head[CAP], tail[CAP];  // elements of the first / last group outside the tensor
 };
+// Partial sums of one call (device memory; the CTAs' sums lie behind it).  A call
+// finds `count` at 0 and leaves it so.
+struct NormSlot {
+  unsigned count, pad_;  // CTAs that have posted their sums
+  double so_far;         // sum of the list's earlier launches
+};
 struct NormArgs {
   int n;                         // tensors in the table (world size 1)
   int first, last;               // first / last launch of the list
@@ -119,7 +125,7 @@ cudaError_t adamw_peers_occupancy(bool quant, cocoDataType_t g_type, int world, 
 
 template <int CAP>
 cudaError_t launch_grad_norm(cocoDataType_t g_type, const NormTable<CAP> &table,
-                             const NormArgs &args, FlagPage *page, int ctas, cudaStream_t stream);
+                             const NormArgs &args, NormSlot *slot, int ctas, cudaStream_t stream);
 int grad_norm_threads();
 int grad_norm_ctas_per_sm();
 int grad_norm_groups_per_warp();  // 16-byte groups a warp takes per pass

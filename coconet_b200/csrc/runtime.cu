@@ -30,6 +30,7 @@
 #include "coconet_fused_generic.cuh"
 #include "fused_step.cuh"
 #include "list_step.cuh"
+#include "norm_slots.h"
 
 using namespace coco;
 
@@ -229,6 +230,7 @@ struct cocoComm {
   size_t seg_part_cap = 0;         // in doubles
   char *list_dev = nullptr;        // AdamW / norm over a list at world sizes above 1: the ranks' pieces
   size_t list_cap = 0;             // in bytes
+  std::shared_ptr<NormSlots> norm_slots;  // gradient norms at world size 1
   int ctas_per_sm = 0;  // 0 = automatic
   int threads = 512;
   int timeout_ms = 10000;
@@ -286,6 +288,14 @@ int init_common(cocoComm *c) {
   // scattered LAMB calls (tensor_norms_of)
   CUDA_TRY(cudaMalloc((void **)&c->flags, kCommPageBytes));
   CUDA_TRY(cudaMemset(c->flags, 0, kCommPageBytes));
+  if (c->world == 1) {
+    try {
+      c->norm_slots = std::make_shared<NormSlots>(std::min(grad_norm_ctas_per_sm() * c->sm_count, kMaxCtasPerRank));
+      CUDA_TRY(c->norm_slots->grow());
+    } catch (...) {
+      return cocoInternalError;
+    }
+  }
   CUDA_TRY(cudaDeviceSynchronize());
   c->peer_flags[c->rank] = c->flags;
   return cocoSuccess;
@@ -922,6 +932,8 @@ template <int CAP> int launch_norm_local(cocoComm *c, const ListCall &lc) {
   static thread_local NormTable<CAP> tab;
   const size_t es = dtype_size(lc.g_type), per = 16 / es;
   NormArgs a = lc.norm;
+  NormSlot *slot = nullptr;
+  CUDA_TRY(c->norm_slots->of(lc.stream, &slot));
   size_t b = 0, part = 0;  // part: groups of tensor b that earlier entries hold
   a.first = 1;
   do {
@@ -949,7 +961,7 @@ template <int CAP> int launch_norm_local(cocoComm *c, const ListCall &lc) {
     a.n = n;
     a.last = b >= lc.n;
     const size_t units = (at + grad_norm_groups_per_warp() - 1) / grad_norm_groups_per_warp();
-    CUDA_TRY(launch_grad_norm<CAP>(lc.g_type, tab, a, c->flags, ctas_for(c, units, grad_norm_threads(), grad_norm_ctas_per_sm()),
+    CUDA_TRY(launch_grad_norm<CAP>(lc.g_type, tab, a, slot, ctas_for(c, units, grad_norm_threads(), grad_norm_ctas_per_sm()),
                                    lc.stream));
     c->launches++;
     a.first = 0;
@@ -1487,8 +1499,10 @@ int cocoCommInitAll(cocoComm_t *comms, int n, const int *devices) {
     }
   cudaSetDevice(prev);
   if (rc != cocoSuccess) {
-    for (auto &c : made)
+    for (auto &c : made) {
+      if (c->norm_slots) c->norm_slots->destroy();
       if (c->flags) cudaFree(c->flags);
+    }
     return rc;
   }
   for (int r = 0; r < n; ++r) {
@@ -1534,6 +1548,7 @@ int cocoCommDestroy(cocoComm_t comm) {
         cudaFree(kv.second);
       }
   }
+  if (comm->norm_slots) comm->norm_slots->destroy();
   if (comm->list_dev) cudaFree(comm->list_dev);
   if (comm->seg_part) cudaFree(comm->seg_part);
   if (comm->flags) cudaFree(comm->flags);

@@ -343,9 +343,12 @@ int cocoFusedLAMBScattered(cocoComm_t comm, size_t nbuff, const void *const *g,
  *    list, so it may be captured into a CUDA graph; the scalars are replayed as
  *    they were captured.  Above it a call that is being captured is refused
  *    (cocoInvalidUsage).
- *  - AdamW calls of one communicator may overlap at world size 1; gradient norms
- *    share its partial sums, like any two fused calls.  cocoLastPhaseTimes and
- *    cocoLastCtaSpread do not cover these calls.
+ *  - At world size 1 these calls may overlap one another, on several streams and
+ *    from several captured graphs.  A captured call may not overlap itself, as it
+ *    would in two executable graphs of one capture; a stream's norms and a graph's
+ *    have partial sums of their own.  Above world size 1 the calls of a
+ *    communicator follow one another, like any two fused calls.
+ *    cocoLastPhaseTimes and cocoLastCtaSpread do not cover these calls.
  *
  * cocoGradNormScattered:  norm[0] = |grad_scale| * || sum over ranks of g ||_2
  * over the whole list, norm[1] = max_norm / norm[0] where 0 < max_norm < norm[0]
