@@ -1080,6 +1080,21 @@ int launch_list_peers(cocoComm *c, const ListCall &lc, std::vector<PeerRank> &ra
   return cocoSuccess;
 }
 
+// Whether two ranks ask for the same step: the ranks of a device run with the first
+// one's scalars, and a slice that is clipped, skipped, rounded or decayed differently
+// from the others is no step at all.
+bool same_step(const ListCall &x, const ListCall &y) {
+  const AdamWArgs &a = x.adam, &b = y.adam;
+  if (x.norm.scale != y.norm.scale || x.norm.max_norm != y.norm.max_norm) return false;
+  if ((a.norm != nullptr) != (b.norm != nullptr) || a.lp_kind != b.lp_kind || a.key != b.key) return false;
+  const float p[] = {a.grad_scale, a.beta1, a.beta2, a.omb1, a.omb2, a.neg_c1, a.rs2, a.eps, a.decay};
+  const float q[] = {b.grad_scale, b.beta1, b.beta2, b.omb1, b.omb2, b.neg_c1, b.rs2, b.eps, b.decay};
+  if (memcmp(p, q, sizeof(p)) != 0) return false;
+  for (size_t k = 0; k < x.n; ++k)
+    if (x.counts[k] > 0 && (x.no_decay && x.no_decay[k]) != (y.no_decay && y.no_decay[k])) return false;
+  return true;
+}
+
 // Every rank of a single-process group has called.
 int flush_list_group(LocalGroup *grp) {
   const int R = (int)grp->comms.size();
@@ -1093,7 +1108,7 @@ int flush_list_group(LocalGroup *grp) {
     const ListCall &lc = pc.list->call;
     if (lc.op != first.op || lc.n != first.n || lc.g_type != first.g_type || (lc.lp != nullptr) != (first.lp != nullptr) ||
         lc.lp_type != first.lp_type || pc.sa.seq != seq ||
-        memcmp(lc.counts, first.counts, sizeof(size_t) * first.n) != 0)
+        memcmp(lc.counts, first.counts, sizeof(size_t) * first.n) != 0 || !same_step(lc, first))
       return cocoInvalidUsage;  // ranks disagree on the operation
     flags[r] = grp->comms[r]->flags;
     for (size_t b = 0; b < first.n; ++b) {

@@ -343,6 +343,9 @@ int cocoFusedLAMBScattered(cocoComm_t comm, size_t nbuff, const void *const *g,
  *    list, so it may be captured into a CUDA graph; the scalars are replayed as
  *    they were captured.  Above it a call that is being captured is refused
  *    (cocoInvalidUsage).
+ *  - Every rank passes the same scalars and the same no_decay, and either every rank
+ *    a norm or none.  Ranks of one process that do not are refused
+ *    (cocoInvalidUsage, nothing runs); between processes nothing compares them.
  *  - At world size 1 these calls may overlap one another, on several streams and
  *    from several captured graphs.  A captured call may not overlap itself, as it
  *    would in two executable graphs of one capture; a stream's norms and a graph's

@@ -1,0 +1,87 @@
+"""Ranks of one process calling the operations on lists together: ranks that disagree
+are refused before anything runs."""
+import numpy as np
+import pytest
+import torch
+
+import adamw_ref as A
+
+import coconet_b200 as coco
+
+COUNTS = [1000, 7, 257]
+HYPER = dict(lr=1e-3, beta1=0.9, beta2=0.999, eps=1e-6, weight_decay=0.01)
+
+
+class Ranks:
+    def __init__(self, quant, counts=COUNTS):
+        self.quant = quant
+        self.comms = coco.Communicator.init_all(2, [0, 0])
+        self.ws = [[torch.ones(c, device="cuda") for c in counts] for _ in range(2)]
+        self.gs = [[torch.full((c,), 0.5, device="cuda") for c in counts] for _ in range(2)]
+        if quant:
+            self.state = [coco.quant_state(counts, 2) for _ in range(2)]
+        else:
+            n = coco.scattered_slice_elems(counts, 2)
+            self.state = [tuple(torch.zeros(n, device="cuda") for _ in range(2)) for _ in range(2)]
+
+    def step(self, *by_rank):
+        with coco.group():
+            for r, kw in enumerate(by_rank):
+                kw = dict(HYPER, step=2, grad_scale=1.0, norm=None, no_decay=None, **({"seed": 5} if self.quant else {})) | kw
+                call = self.comms[r].fused_adamw_quant_scattered if self.quant else self.comms[r].fused_adamw_scattered
+                call(self.gs[r], self.ws[r], *self.state[r], **kw)
+
+    def untouched(self):
+        torch.cuda.synchronize()
+        return (all(bool((x == 1).all()) for r in self.ws for x in r) and
+                all(not x.view(torch.uint8).any() for r in self.state for x in r))
+
+
+@pytest.fixture
+def ranks(request):
+    r = Ranks(getattr(request, "param", False))
+    yield r
+    torch.cuda.synchronize()
+    for c in r.comms:
+        c.destroy()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("ranks", [False, True], indirect=True, ids=["fp32", "8-bit"])
+def test_ranks_that_disagree_about_a_step_are_refused(ranks):
+    norm = torch.tensor([2.0, 0.5], device="cuda")
+    cases = [dict(lr=2e-3), dict(beta1=0.8), dict(beta2=0.99), dict(eps=1e-5), dict(weight_decay=0.02), dict(step=3),
+             dict(grad_scale=0.5), dict(norm=norm), dict(no_decay=[True, False, False])]
+    if ranks.quant:
+        cases += [dict(seed=6), dict(seed=5 + (1 << 32))]
+    for kw in cases:
+        for by_rank in (({}, kw), (kw, {})):
+            with pytest.raises(coco.CocoError) as e:
+                ranks.step(*by_rank)
+            assert e.value.code == 2, kw
+            assert ranks.untouched(), kw
+    ranks.step(dict(norm=norm, no_decay=[False] * 3), dict(norm=norm.clone()))   # the same in other words
+    assert not ranks.untouched()
+    assert all(torch.equal(a, b) for a, b in zip(*ranks.ws))
+    assert all(c.status()["code"] == 0 for c in ranks.comms)
+
+
+@pytest.mark.gpu
+def test_ranks_that_disagree_about_a_norm_are_refused(ranks):
+    outs = [torch.full((2,), -1.0, device="cuda") for _ in range(2)]
+
+    def norm(*by_rank):
+        with coco.group():
+            for r, kw in enumerate(by_rank):
+                ranks.comms[r].grad_norm_scattered(ranks.gs[r], outs[r], **kw)
+    for kw in (dict(max_norm=1.0), dict(grad_scale=0.5)):
+        for by_rank in (({}, kw), (kw, {})):
+            with pytest.raises(coco.CocoError) as e:
+                norm(*by_rank)
+            assert e.value.code == 2, kw
+    torch.cuda.synchronize()
+    assert all(bool((o == -1).all()) for o in outs)
+    norm(dict(max_norm=1.0), dict(max_norm=1.0))
+    n = float(np.sqrt(sum(COUNTS)))     # the sum of the two gradients is 1 everywhere
+    for o in outs:
+        assert abs(float(o[0]) - n) <= 1.1 * A.U * n and abs(float(o[1]) - 1 / n) <= 2.1 * A.U / n
