@@ -693,7 +693,12 @@ int flush_group(LocalGroup *grp) {
       return cocoInvalidUsage;  // ranks disagree on the operation
     }
   if (first.list) {
-    const int rc = flush_list_group(grp);
+    int rc;
+    try {
+      rc = flush_list_group(grp);
+    } catch (...) {  // the host ran out of memory; cocoGroupEnd is a C entry point
+      rc = cocoInternalError;
+    }
     for (cocoComm *c : grp->comms) c->has_pending = false, c->pending.list.reset();
     return rc;
   }
@@ -1177,13 +1182,13 @@ int enqueue_list_or_throw(cocoComm *c, ListCall &lc) {
     COCO_TRY(refuse_capture(c, lc.stream));
     c->pending = PendingCall();
     c->pending.list = std::make_shared<OwnedListCall>(lc);
+    if (g_group_depth > 0 &&
+        std::find(g_group_touched.begin(), g_group_touched.end(), c) == g_group_touched.end())
+      g_group_touched.push_back(c);
+    // nothing below can throw but the launch, which forgets the pending calls if it does
     c->pending.sa.seq = ++c->seq;
     c->has_pending = true;
-    if (g_group_depth > 0) {
-      if (std::find(g_group_touched.begin(), g_group_touched.end(), c) == g_group_touched.end())
-        g_group_touched.push_back(c);
-      return cocoSuccess;
-    }
+    if (g_group_depth > 0) return cocoSuccess;
     for (cocoComm *o : c->group->comms)
       if (!o->has_pending) return cocoSuccess;  // more ranks to come
     return flush_group(c->group.get());

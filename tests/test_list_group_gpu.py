@@ -1,5 +1,10 @@
 """Ranks of one process calling the operations on lists together: ranks that disagree
-are refused before anything runs."""
+are refused before anything runs, and a host that runs out of memory leaves the group
+usable."""
+import os
+import subprocess
+import sys
+
 import numpy as np
 import pytest
 import torch
@@ -8,6 +13,7 @@ import adamw_ref as A
 
 import coconet_b200 as coco
 
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 COUNTS = [1000, 7, 257]
 HYPER = dict(lr=1e-3, beta1=0.9, beta2=0.999, eps=1e-6, weight_decay=0.01)
 
@@ -85,3 +91,47 @@ def test_ranks_that_disagree_about_a_norm_are_refused(ranks):
     n = float(np.sqrt(sum(COUNTS)))     # the sum of the two gradients is 1 everywhere
     for o in outs:
         assert abs(float(o[0]) - n) <= 1.1 * A.U * n and abs(float(o[1]) - 1 / n) <= 2.1 * A.U / n
+
+
+OUT_OF_MEMORY = f"""
+import ctypes as C, sys
+sys.path[:0] = [{os.path.dirname(os.path.abspath(__file__))!r}, {ROOT!r}]
+import torch, coconet_b200 as coco
+from test_list_group_gpu import Ranks
+shim = C.CDLL(sys.argv[1])
+shim.new_fails_at.argtypes = [C.c_size_t, C.c_int]
+ranks = Ranks(sys.argv[2] == "8-bit", [100] * 41)
+failed = 0
+for skip in range(64):
+    # the tables that a launch is made from hold 24 bytes for each of the 41 tensors
+    shim.new_fails_at(24 * 41, skip)
+    try:
+        ranks.step({{}}, {{}})
+        code = 0
+    except coco.CocoError as e:
+        code = e.code
+    hit = shim.new_failed()
+    shim.new_fails_at(0, 0)
+    assert code == (7 if hit else 0), (skip, code, hit)
+    if not hit:
+        break
+    failed += 1
+    assert ranks.untouched(), skip
+assert failed > 0
+torch.cuda.synchronize()
+assert not ranks.untouched()
+ranks.step({{}}, {{}})                 # and once more, as ever
+torch.cuda.synchronize()
+assert all(c.status()["code"] == 0 for c in ranks.comms)
+print("failed", failed)
+"""
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("form", ["fp32", "8-bit"])
+def test_a_host_out_of_memory_leaves_the_group_usable(tmp_path, form):
+    shim = str(tmp_path / "new_fails.so")
+    subprocess.check_call(["g++", "-O1", "-fPIC", "-shared", os.path.join(ROOT, "tests", "new_fails.cpp"), "-o", shim])
+    r = subprocess.run([sys.executable, "-c", OUT_OF_MEMORY, shim, form], env=dict(os.environ, LD_PRELOAD=shim),
+                       capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0, r.stdout[-2000:] + r.stderr[-3000:]
