@@ -1100,6 +1100,18 @@ bool same_step(const ListCall &x, const ListCall &y) {
   return true;
 }
 
+// Makes what comes on `later` wait for what is on `earlier`.
+int order_streams(cudaStream_t earlier, cudaStream_t later) {
+  if (earlier == later) return cocoSuccess;
+  cudaEvent_t done;
+  CUDA_TRY(cudaEventCreateWithFlags(&done, cudaEventDisableTiming));
+  cudaError_t e = cudaEventRecord(done, earlier);
+  if (e == cudaSuccess) e = cudaStreamWaitEvent(later, done, 0);
+  cudaEventDestroy(done);  // (its wait stays)
+  CUDA_TRY(e);
+  return cocoSuccess;
+}
+
 // Every rank of a single-process group has called.
 int flush_list_group(LocalGroup *grp) {
   const int R = (int)grp->comms.size();
@@ -1134,7 +1146,12 @@ int flush_list_group(LocalGroup *grp) {
       pieces.push_back(build_peer_pieces(c->rank, R, L, lc, g, out));
       ranks.push_back(peer_rank_of(c, lc, L, flags, pieces.back()));
     }
-    COCO_TRY(launch_list_peers(kv.second[0], kv.second[0]->pending.list->call, ranks, pieces, L.slice, seq));
+    // one launch for the ranks of this device: behind what each has on its own stream,
+    // and before what each enqueues there next
+    const ListCall &lead = kv.second[0]->pending.list->call;
+    for (cocoComm *c : kv.second) COCO_TRY(order_streams(c->pending.list->call.stream, lead.stream));
+    COCO_TRY(launch_list_peers(kv.second[0], lead, ranks, pieces, L.slice, seq));
+    for (cocoComm *c : kv.second) COCO_TRY(order_streams(lead.stream, c->pending.list->call.stream));
   }
   return cocoSuccess;
 }

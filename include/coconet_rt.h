@@ -346,6 +346,8 @@ int cocoFusedLAMBScattered(cocoComm_t comm, size_t nbuff, const void *const *g,
  *  - Every rank passes the same scalars and the same no_decay, and either every rank
  *    a norm or none.  Ranks of one process that do not are refused
  *    (cocoInvalidUsage, nothing runs); between processes nothing compares them.
+ *  - A rank's part follows what is on the stream it passed and precedes what it
+ *    enqueues there next, ranks of one process on one GPU with a stream each included.
  *  - At world size 1 these calls may overlap one another, on several streams and
  *    from several captured graphs.  A captured call may not overlap itself, as it
  *    would in two executable graphs of one capture; a stream's norms and a graph's

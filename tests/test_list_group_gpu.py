@@ -93,6 +93,58 @@ def test_ranks_that_disagree_about_a_norm_are_refused(ranks):
         assert abs(float(o[0]) - n) <= 1.1 * A.U * n and abs(float(o[1]) - 1 / n) <= 2.1 * A.U / n
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("late", [0, 1])
+@pytest.mark.parametrize("op", ["norm", "fp32", "8-bit"])
+def test_ranks_of_one_gpu_with_a_stream_each(op, late):
+    """The gradients of one rank come late on its stream, and its stream reads the results at once."""
+    counts = [70001, 513, 9]
+    ranks = Ranks(op == "8-bit", counts)
+    try:
+        streams = [torch.cuda.Stream() for _ in range(2)]
+        outs = [torch.zeros(2, device="cuda") for _ in range(2)]
+        a = torch.ones(4096, 4096, device="cuda")
+        b = torch.empty_like(a)
+        seen = [None, None]
+        for value in (1.5, 3.5):
+            torch.cuda.synchronize()
+            with torch.cuda.stream(streams[late]):
+                for _ in range(20):             # some milliseconds
+                    torch.matmul(a, a, out=b)
+                for g in ranks.gs[late]:
+                    g.fill_(value)
+            with coco.group():
+                for r in range(2):
+                    if op == "norm":
+                        ranks.comms[r].grad_norm_scattered(ranks.gs[r], outs[r], stream=streams[r])
+                    elif op == "fp32":
+                        ranks.comms[r].fused_adamw_scattered(ranks.gs[r], ranks.ws[r], *ranks.state[r], **HYPER, step=0,
+                                                             stream=streams[r])
+                    else:
+                        ranks.comms[r].fused_adamw_quant_scattered(ranks.gs[r], ranks.ws[r], *ranks.state[r], **HYPER,
+                                                                   step=0, seed=1, stream=streams[r])
+            for r in range(2):
+                with torch.cuda.stream(streams[r]):
+                    seen[r] = [x.clone() for x in (outs[r:r + 1] if op == "norm" else ranks.ws[r])]
+                    for g in ranks.gs[r]:
+                        g.fill_(0.5)            # the next step's, while the other rank may still be at it
+            torch.cuda.synchronize()
+            if op == "norm":
+                n = (0.5 + value) * sum(counts) ** 0.5
+                assert all(abs(float(s[0][0]) - n) <= 1.1 * A.U * n for s in seen)
+            else:
+                assert all(torch.equal(x, y) for r in range(2) for x, y in zip(seen[r], ranks.ws[r]))
+                assert all(torch.equal(x, y) for x, y in zip(*ranks.ws))
+        if op == "fp32":    # both steps saw the late gradients: m = 0.1 (0.9 * 2 + 4), where the fp32 number
+            m = torch.cat([x for r in ranks.state for x in r[:1]])   # 1 - 0.9 is 4 u off, and four roundings more
+            assert abs(float(m.max()) - 0.58) <= 8 * A.U * 0.58
+        assert all(c.status()["code"] == 0 for c in ranks.comms)
+    finally:
+        torch.cuda.synchronize()
+        for c in ranks.comms:
+            c.destroy()
+
+
 OUT_OF_MEMORY = f"""
 import ctypes as C, sys
 sys.path[:0] = [{os.path.dirname(os.path.abspath(__file__))!r}, {ROOT!r}]
