@@ -1067,6 +1067,7 @@ cudaError_t launch_adamw_peers(bool quant, cocoDataType_t g_type, const PeerArgs
     return cudaLaunchCooperativeKernel((const void *)k, grid, dim3(cfg.threads), params, 0, stream);
   return cudaLaunchKernel((const void *)k, grid, dim3(cfg.threads), params, 0, stream);
 }
+int adamw_peer_threads() { return COCO_ADAMW_PEER_THREADS; }
 cudaError_t adamw_peers_occupancy(bool quant, cocoDataType_t g_type, int world, int threads,
                                   int *ctas_per_sm) {
   const PeerKernel k = pick_peer(quant, g_type, world);

@@ -120,6 +120,7 @@ cudaError_t launch_adamw(bool quant, bool packed, cocoDataType_t g_type, const L
 unsigned adamw_rounding_key(uint64_t seed, int step);
 cudaError_t launch_adamw_peers(bool quant, cocoDataType_t g_type, const PeerArgs &peers,
                                const AdamWArgs &args, const ListLaunch &cfg, cudaStream_t stream);
+int adamw_peer_threads();
 cudaError_t adamw_peers_occupancy(bool quant, cocoDataType_t g_type, int world, int threads,
                                   int *ctas_per_sm);
 

@@ -1068,7 +1068,7 @@ int launch_list_peers(cocoComm *c, const ListCall &lc, std::vector<PeerRank> &ra
   pa.timeout_ns = (unsigned long long)c->timeout_ms * 1000000ull;
   ListLaunch cfg = {};
   const bool norm = lc.op == kListGradNorm, quant = lc.op == kListAdamWQuant;
-  cfg.threads = norm ? grad_norm_threads() : 256;
+  cfg.threads = norm ? grad_norm_threads() : adamw_peer_threads();
   cfg.nvirt = nvirt;
   cfg.cooperative = nvirt > 1;
   if (cfg.cooperative && !c->coop_supported) return cocoInvalidUsage;

@@ -33,7 +33,7 @@ int main(int argc, char **argv) {
   const bool in_time = argc > 2 && !strcmp(argv[2], "in-time");
   cudaDeviceProp prop;
   CHECK(cudaGetDeviceProperties(&prop, 0));
-  const int threads = norm ? grad_norm_threads() : 256;
+  const int threads = norm ? grad_norm_threads() : adamw_peer_threads();
   int occ = 0;
   CHECK(norm ? grad_norm_peers_occupancy(cocoFloat32, 2, threads, &occ)
              : adamw_peers_occupancy(quant, cocoFloat32, 2, threads, &occ));
