@@ -8,7 +8,7 @@ CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libcoconet_rt.so")
 SOURCES = ["fused_step.cu", "runtime.cu", "bootstrap.cpp", "no_alloc.cu", "symm_mem.cu", "collectives.cu",
            "link_probe.cu", "adamw.cu", "grad_norm.cu"]
-HEADERS = ["fused_step.cuh", "device_util.cuh", "list_step.cuh", "list_device.cuh", "norm_slots.h", "bootstrap.h", os.path.join(ROOT, "include", "coconet_rt.h"),
+HEADERS = ["fused_step.cuh", "device_util.cuh", "list_step.cuh", "list_device.cuh", "pair_math.cuh", "norm_slots.h", "bootstrap.h", os.path.join(ROOT, "include", "coconet_rt.h"),
            os.path.join(ROOT, "include", "coconet_device.h"),
            os.path.join(ROOT, "include", "coconet_fused_generic.cuh")]
 NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
