@@ -330,6 +330,7 @@ class TensorList:
         self._at = tuple(C.addressof(x) if x is not None else None
                          for x in (self.g, self.w, self.lp, self.counts, self.no_decay))
         self._device = None   # set once the list has passed _checked
+        self._distinct = False   # and this, once what an AdamW call writes has
         self._slices = {}
 
     def _checked(self, weights):
@@ -338,6 +339,12 @@ class TensorList:
         gs, ws, lps = self.tensors
         if weights and ws is None:
             raise ValueError("this list holds no weights")
+        if weights and not self._distinct:
+            for what, at in (("weight", self.w), ("low-precision copy", self.lp)):
+                held = [p for p, count in zip(at or (), self.counts) if count]
+                if len(set(held)) != len(held):   # e.g. tied weights: two updates would meet in one place
+                    raise ValueError(f"the list holds a {what} twice")
+            self._distinct = True
         if self._device is None:
             import torch
             dev = gs[0].device

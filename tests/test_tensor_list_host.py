@@ -44,3 +44,27 @@ def test_a_tensor_list_by_itself_goes_on_to_the_other_checks(quant):
         _call(comm, quant, lst, ws=[w], w_lps=[lp], no_decay=[1])
     with pytest.raises(ValueError, match="CUDA"):   # and plain lists keep their arguments
         _call(comm, quant, [torch.zeros(256)], [torch.zeros(256)], no_decay=[True], w_lps=[torch.zeros(256).half()])
+
+
+@pytest.mark.parametrize("what", ["weight", "copy"])
+def test_a_tensor_that_is_written_twice_is_refused(what):
+    comm = coco.Communicator(None, 1, 0)
+    g, w, lp = ([torch.zeros(64) for _ in range(2)] for _ in range(3))
+    lp = [x.half() for x in lp]
+    if what == "weight":
+        w[1] = w[0]
+    else:
+        lp[1] = lp[0].view(8, 8)
+    with pytest.raises(ValueError, match=f"{what} twice"):
+        comm.fused_adamw_scattered(g, w, w[0], w[0], *HYPER, w_lps=lp)
+    lst = coco.TensorList([g[0], g[0]], w, lps=lp)
+    with pytest.raises(ValueError, match="CUDA"):   # the norm writes neither, and a gradient may be there twice
+        comm.grad_norm_scattered(lst, torch.zeros(2))
+    with pytest.raises(ValueError, match=f"{what} twice"):
+        comm.fused_adamw_scattered(lst, None, w[0], w[0], *HYPER)
+
+
+def test_empty_tensors_may_be_there_twice():
+    e, t = torch.zeros(0), [torch.zeros(64) for _ in range(4)]
+    with pytest.raises(ValueError, match="CUDA"):
+        coco.Communicator(None, 1, 0).fused_adamw_scattered([t[0], e, e], [t[1], e, e], t[2], t[3], *HYPER)
