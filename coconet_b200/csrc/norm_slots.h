@@ -52,7 +52,9 @@ class NormSlots : public std::enable_shared_from_this<NormSlots> {
     for (char *c : chunks_) cudaFree(c);
     if (fill_) cudaStreamDestroy(fill_);
     chunks_.clear(), free_.clear(), by_stream_.clear();
-    fill_ = nullptr, closed_ = true;
+    fill_ = nullptr;
+    std::lock_guard<std::mutex> lock_back(back_mu_);
+    back_.clear(), closed_ = true;
   }
 
   cudaError_t grow() {  // by one chunk; allowed while a stream is being captured
@@ -70,7 +72,10 @@ class NormSlots : public std::enable_shared_from_this<NormSlots> {
       return e;
     }
     chunks_.push_back(chunk);
-    free_.reserve(chunks_.size() * kChunk);  // giving one back allocates nothing
+    {
+      std::lock_guard<std::mutex> lock_back(back_mu_);
+      back_.reserve(chunks_.size() * kChunk);  // giving one back allocates nothing
+    }
     for (int k = kChunk - 1; k >= 0; --k) free_.push_back((NormSlot *)(chunk + slot_bytes_ * k));
     return cudaSuccess;
   }
@@ -83,13 +88,20 @@ class NormSlots : public std::enable_shared_from_this<NormSlots> {
     std::shared_ptr<NormSlots> owner;
     NormSlot *slot;
   };
-  static void CUDART_CB give_back(void *p) {  // the last graph that holds the call is gone
+  // The last graph that holds the call is gone.  Runs on a thread of the CUDA runtime
+  // and so takes no lock that is held across calls into it.
+  static void CUDART_CB give_back(void *p) {
     std::unique_ptr<Captured> c((Captured *)p);
-    std::lock_guard<std::mutex> lock(c->owner->mu_);
-    if (!c->owner->closed_) c->owner->free_.push_back(c->slot);
+    std::lock_guard<std::mutex> lock_back(c->owner->back_mu_);
+    if (!c->owner->closed_) c->owner->back_.push_back(c->slot);
   }
 
   cudaError_t take(NormSlot **out) {
+    {
+      std::lock_guard<std::mutex> lock_back(back_mu_);
+      free_.insert(free_.end(), back_.begin(), back_.end());
+      back_.clear();
+    }
     if (free_.empty()) {
       const cudaError_t e = grow();
       if (e != cudaSuccess) return e;
@@ -131,6 +143,8 @@ class NormSlots : public std::enable_shared_from_this<NormSlots> {
   std::vector<NormSlot *> free_;
   std::map<unsigned long long, NormSlot *> by_stream_;
   cudaStream_t fill_ = nullptr;
+  std::mutex back_mu_;            // of what follows; taken last
+  std::vector<NormSlot *> back_;  // slots of graphs that are gone
   bool closed_ = false;
 };
 
