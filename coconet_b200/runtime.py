@@ -341,7 +341,9 @@ class TensorList:
             raise ValueError("this list holds no weights")
         if weights and not self._distinct:
             for what, at in (("weight", self.w), ("low-precision copy", self.lp)):
-                held = [p for p, count in zip(at or (), self.counts) if count]
+                if at is None or len(set(at[:])) == self.n:
+                    continue
+                held = [p for p, count in zip(at, self.counts) if count]   # without empty tensors
                 if len(set(held)) != len(held):   # e.g. tied weights: two updates would meet in one place
                     raise ValueError(f"the list holds a {what} twice")
             self._distinct = True
