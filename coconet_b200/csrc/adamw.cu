@@ -140,7 +140,7 @@ __device__ __forceinline__ void update1(const AdamWArgs &a, float decay, float g
 
 // ---- 8-bit codes -----------------------------------------------------------------
 // With 8-bit moments the instructions, not the bytes, bound the kernel (156 per
-// element in the first form, 67 now; 88 would fill every issue slot at the copy rate):
+// element in the first form, 66 now; 88 would fill every issue slot at the copy rate):
 // two elements per instruction (f32x2) where there is a form for it.
 
 // Multiply and xor-shift rounds; the multipliers are binary fractions of the
@@ -557,12 +557,17 @@ __global__ void __launch_bounds__(COCO_ADAMW_THREADS, 2)
 // below its start to the one above its end (memory of the same allocation), and its new
 // weights leave through shared memory, in 16-byte stores but for the ends of a unit.
 // Where a tile holds several tensors its units are copied one by one.
-//  8-bit moments, 336 M elements (16 bytes each): 0.83 ms, 0.99 of the copy rate, in a
+//  (Times of the kernel alone, from a captured graph.)
+//  8-bit moments, 336 M elements (16 bytes each): 0.84 ms, 0.98 of the copy rate, in a
 //  burst, 0.92 ms at the clocks of a long run; with four tiles in flight in place of three
 //  0.92.  With two CTAs per SM 0.88 ms in a burst, and beside that: loads by the threads
 //  themselves 0.94 ms, asynchronous copies by every warp for itself 1.20 ms (102
 //  instructions per element), L2 prefetches one to three units ahead 1.02 to 1.07 ms; two
 //  tiles in flight 1.01, four 0.91 ms; 16, 14, 11, 10 warps 0.91, 0.91, 0.98, 0.91 ms.
+//  8-bit moments, 900 tensors, 29 M elements: 80 us aligned, 96 packed (0.73).  Those are
+//  read and written in shared memory element by element, up to four lanes to a bank: four
+//  times the wavefronts of the aligned ones, 60 % of the shared memory's cycles, while the
+//  issue slots are busy for 66 % (aligned: 72 %).
 //  fp32 moments, 900 tensors, 29 M elements, hardly one aligned: 138 us (0.90) against
 //  146 us with element by element loads and stores; 30 such tensors of fp32 gradients,
 //  21 M elements: 101 us (0.94).  8 and 9 warps with three tiles in flight 141 and 146 us,
@@ -934,7 +939,7 @@ template <bool QUANT, bool WIDE, typename GT, int CAP> Kernel<CAP> pick_staged(L
 }
 // 8-bit moments: staged tiles, which measured better for aligned tensors too.  `wide`,
 // one CTA of 24 warps per SM in place of two of 12, has half as many tiles: better where
-// they lie in one tensor mostly (398 tensors, 336 M elements: 0.83 against 0.88 ms; 30
+// they lie in one tensor mostly (398 tensors, 336 M elements: 0.84 against 0.88 ms; 30
 // tensors, 21 M: 56.5 against 57.5 us), worse where many hold several (900 tensors, 29 M:
 // 84 against 80 us, packed 102 against 96) and on few tiles (one tensor of 256 Ki elements
 // 5.0 against 3.8 us, of 1 Mi 7.4 against 6.0; of 4 Mi the same, of 16 Mi 46.6 against 47.1).

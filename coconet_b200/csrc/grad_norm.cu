@@ -6,8 +6,9 @@
 // What bounds it: reading g once from HBM (2 or 4 bytes per element, a
 // conversion and a multiply-add each): 336 M fp32 elements 193 us, 1.06 of the
 // measured copy rate (reads alone are faster than a copy); a list of 12.6 M bf16
-// elements 7.1 us, of which 2.5 us are an empty call's.  Three CTAs of 512 threads
-// with four 16-byte loads each: two CTAs with eight 255 us, four with four 216 us.  Squares are added in fp32 within 16
+// elements 7.0 us, of which 2.5 us are an empty call's (from a captured graph).  Three
+// CTAs of 512 threads with four 16-byte loads each: two CTAs with eight 255 us, four with
+// four 216 us.  Squares are added in fp32 within 16
 // bytes only and in fp64 from there on, in an order fixed by the launch shape:
 // repeated calls give the same bits.  Where 16 bytes' sum leaves the range in
 // which fp32 loses nothing that matters, it is redone in fp64.

@@ -338,11 +338,14 @@ int cocoFusedLAMBScattered(cocoComm_t comm, size_t nbuff, const void *const *g,
  *    Gradients, weights, copies and state must not overlap one another.
  *  - Elements need only the alignment of their type; tensors that start on 16
  *    bytes are faster.  The aligned 16 bytes in which a gradient or weight tensor
- *    begins and ends may be read as a whole (not written).
+ *    or the array of scales begins and ends may be read as a whole (not written).
  *  - World size 1: a call is one kernel per 1024 tensors and keeps nothing of the
  *    list, so it may be captured into a CUDA graph; the scalars are replayed as
  *    they were captured.  Above it a call that is being captured is refused
  *    (cocoInvalidUsage).
+ *  - A rank that waits for a late one gives up after the communicator's time limit:
+ *    its status word says so, its norm is nan, and of a step what was not done is left
+ *    as it was and not announced, so that the other ranks' status words say so too.
  *  - Every rank passes the same scalars and the same no_decay, and either every rank
  *    a norm or none.  Ranks of one process that do not are refused
  *    (cocoInvalidUsage, nothing runs); between processes nothing compares them.
@@ -350,25 +353,28 @@ int cocoFusedLAMBScattered(cocoComm_t comm, size_t nbuff, const void *const *g,
  *    enqueues there next, ranks of one process on one GPU with a stream each included.
  *  - At world size 1 these calls may overlap one another, on several streams and
  *    from several captured graphs.  A captured call may not overlap itself, as it
- *    would in two executable graphs of one capture; a stream's norms and a graph's
- *    have partial sums of their own.  Above world size 1 the calls of a
- *    communicator follow one another, like any two fused calls.
+ *    would in two executable graphs of one capture, nor be replayed when the
+ *    communicator is gone; a stream's norms and a graph's have partial sums of their
+ *    own.  Above world size 1 the calls of a communicator follow one another, like
+ *    any two fused calls.
  *    cocoLastPhaseTimes and cocoLastCtaSpread do not cover these calls.
  *
  * cocoGradNormScattered:  norm[0] = |grad_scale| * || sum over ranks of g ||_2
  * over the whole list, norm[1] = max_norm / norm[0] where 0 < max_norm < norm[0]
  * and 1 elsewhere (max_norm <= 0: never clip), 0 where norm[0] is inf or nan.
  * `norm`: two fp32 in this GPU's memory, the same values on every rank.  The sum
- * is held in fp64 and its order is fixed per launch shape, so repeated calls
- * agree to the last bit.
+ * is held in fp64 (the squares of 16 bytes are added in fp32 first where that is safe)
+ * and its order is fixed per launch shape, so repeated calls agree to the last bit.
  *
  * cocoFusedAdamWScattered, with d1 = 1 - beta1^(step+1), d2 = 1 - beta2^(step+1):
  *     g <- (sum over ranks of g) * (norm ? norm[1] * grad_scale : grad_scale)
  *     m <- beta1 m + (1 - beta1) g        v <- beta2 v + (1 - beta2) g^2
  *     w <- w (1 - lr weight_decay) - (lr / d1) m / (sqrt(v) / sqrt(d2) + eps)
  * every operation rounded to fp32 (m and v so to the last bit); the root and the
- * reciprocal in w's update are the hardware's, within 2^-23 each.  With `norm` (as cocoGradNormScattered left it
- * on every rank) whose norm[0] is inf or nan the step changes nothing.
+ * reciprocal in w's update are the hardware's, within 2^-23 each (with 8-bit moments
+ * the root is the rounded one, and the divisor and the last difference are one
+ * multiply-add each).  With `norm` (as cocoGradNormScattered left it on every rank)
+ * whose norm[0] is inf or nan the step changes nothing.
  *   w_lp      NULL, or per tensor a 16-bit copy of w (lp_type), gathered instead
  *             of w; then, as in the flat call, only the own slice of w is updated
  *   no_decay  NULL, or per tensor a byte (host): not 0 = weight_decay does not apply
