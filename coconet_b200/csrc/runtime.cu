@@ -259,7 +259,8 @@ struct DeviceGuard {
   bool ok = true;
   explicit DeviceGuard(int dev) {
     if (cudaGetDevice(&prev) != cudaSuccess) ok = false;
-    if (ok && prev != dev && cudaSetDevice(dev) != cudaSuccess) ok = false;
+    if (prev == dev) prev = -1;  // nothing to change, nothing to put back
+    else if (ok && cudaSetDevice(dev) != cudaSuccess) ok = false;
   }
   ~DeviceGuard() {
     if (prev >= 0) cudaSetDevice(prev);

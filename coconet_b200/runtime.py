@@ -245,6 +245,19 @@ def group():
         _check(lib().cocoGroupEnd(), "cocoGroupEnd")
 
 
+_torch_module = None
+
+
+def _torch():
+    """torch, imported at the first use (the library loads without it); the import
+    statement itself costs 0.2 us, which a small call would pay several times."""
+    global _torch_module
+    if _torch_module is None:
+        import torch
+        _torch_module = torch
+    return _torch_module
+
+
 def _dtype_code(t):
     import torch
     return {torch.float32: _F32, torch.float16: _F16, torch.bfloat16: _BF16}[t.dtype]
@@ -553,7 +566,7 @@ class Communicator:
     def _on(self, device, stream):
         """The stream to use: `stream`, or the current one of the list's device,
         which has to be this communicator's."""
-        import torch
+        torch = _torch()
         if self._device is None:
             d = C.c_int()
             _check(lib().cocoCommCuDevice(self._h, C.byref(d)), "cocoCommCuDevice")
@@ -587,7 +600,7 @@ class Communicator:
         """norm[0] = |grad_scale| * the 2-norm of the summed gradients of the list,
         norm[1] = the factor that clips it to max_norm (<= 0: 1).  `norm`: two
         fp32 on the device; pass it to the AdamW calls."""
-        import torch
+        torch = _torch()
         lst = gs if isinstance(gs, TensorList) else TensorList(gs, None)
         device = lst._checked(weights=False)
         p = self._held(norm, "norm", device, (torch.float32,), 2)
@@ -601,7 +614,7 @@ class Communicator:
         the gradients are scaled by norm[1], and a norm that is not finite skips
         the step.  A TensorList brings its weights, copies and no_decay; other `ws`,
         `w_lps` or `no_decay` beside it are refused."""
-        import torch
+        torch = _torch()
         lst = self._list_of(gs, ws, w_lps, no_decay)
         device = lst._checked(weights=True)
         need, f32 = lst._slice(self.world, False), (torch.float32,)
@@ -618,7 +631,7 @@ class Communicator:
                                     stream=None):
         """AdamW over a list with 8-bit moments (see quant_state): e4m3 codes of m
         and sqrt(v), rounded at random from `seed` and `step`.  A TensorList as above."""
-        import torch
+        torch = _torch()
         lst = self._list_of(gs, ws, w_lps, no_decay)
         device = lst._checked(weights=True)
         need = lst._slice(self.world, True)
