@@ -88,8 +88,9 @@ class NormSlots : public std::enable_shared_from_this<NormSlots> {
     std::shared_ptr<NormSlots> owner;
     NormSlot *slot;
   };
-  // The last graph that holds the call is gone.  Runs on a thread of the CUDA runtime
-  // and so takes no lock that is held across calls into it.
+  // The last graph that holds the call is gone, and its launches have finished: the
+  // runtime keeps the object until then.  Runs on a thread of the runtime and so takes
+  // no lock that is held across calls into it.
   static void CUDART_CB give_back(void *p) {
     std::unique_ptr<Captured> c((Captured *)p);
     std::lock_guard<std::mutex> lock_back(c->owner->back_mu_);

@@ -145,6 +145,37 @@ def test_graphs_give_their_memory_back(comm):  # noqa: F811
     assert float(out[0]) > 0
 
 
+def test_graphs_that_go_while_they_run(comm):  # noqa: F811
+    """A graph is thrown away while its launch still waits its turn; what comes meanwhile does not get its memory."""
+    lists = _lists()
+    expect = _alone(comm, lists)
+    a = torch.ones(4096, 4096, device="cuda")
+    b = torch.empty_like(a)
+    torch.matmul(a, a, out=b)
+    side, other = torch.cuda.Stream(), torch.cuda.Stream()
+    for _ in range(10):
+        outs = torch.zeros(2 * len(lists), 2, device="cuda")
+        torch.cuda.synchronize()
+        for k, lst in enumerate(lists):
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph):
+                comm.grad_norm_scattered(lst, outs[2 * k], max_norm=0.5)
+            with torch.cuda.stream(side):
+                for _ in range(5):
+                    torch.matmul(a, a, out=b)
+                graph.replay()
+            graph.reset()
+            again = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(again):
+                comm.grad_norm_scattered(lst, outs[2 * k + 1], max_norm=0.5)
+            with torch.cuda.stream(other):
+                again.replay()
+            again.reset()
+        torch.cuda.synchronize()
+        for k, e in enumerate(expect):
+            assert torch.equal(outs[2 * k], e) and torch.equal(outs[2 * k + 1], e)
+
+
 def test_more_live_graphs_than_a_first_chunk_holds(comm):  # noqa: F811
     lst = _lists()[2]
     outs = [torch.zeros(2, device="cuda") for _ in range(200)]
